@@ -40,7 +40,7 @@ extern "C" {
  * added.  5: unirl_sde_replay_logp, unirl_sde_replay_logp_bwd, unirl_lmhead_logp added.
  * 6: the unirl_calib_* measurement aids left the library (they live in the measurement build);
  * unirl_flowdppo_replay_step added; in-kernel sampling noise (struct unirl_rng in
- * unirl_sde_step_desc, two more arguments of unirl_sde_rollout_logp). */
+ * unirl_sde_step_desc, two more arguments of unirl_sde_rollout_logp); since then only additions. */
 #define UNIRL_ABI_VERSION 6
 
 enum unirl_dtype { UNIRL_F32 = 0, UNIRL_BF16 = 1, UNIRL_F16 = 2 };
@@ -606,6 +606,132 @@ int unirl_gather_steps(const void* src, int64_t B, int64_t S, int64_t inner_byte
  * ---------------------------------------------------------------------- */
 int unirl_expand_groups(const float* src, int64_t U, int64_t D, const int64_t* group_of, int64_t B,
                         void* out, int out_dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Layer norm / RMS norm in front of a policy's output: the final norm whose output the head reads
+ * (the hidden states of unirl/models/qwen3/ar.py:82-99), and the norm with a gain and a bias per
+ * sample in front of the projection that makes a diffusion policy's velocities
+ * (unirl/models/sd3/diffusion.py:467-497).
+ *   mu = mean(x), s = 1 / sqrt(mean((x - mu)^2) + eps)   (center == 0: mu = 0)
+ *   y = (x - mu) s (gain_offset + gain) + bias
+ * x is [groups, rows, D] with the elements of a row adjacent; y dense in x's dtype, rounded once from
+ * f32.  gain, bias: NULL, or [D] (group stride 0), or one row per group, of one dtype.  mean, rstd:
+ * f32 [groups, rows] outputs, each may be NULL.  D <= 32768.
+ * ---------------------------------------------------------------------- */
+struct unirl_norm_desc {
+  const void* x;
+  int dtype;                                /* unirl_dtype of x, y, dy, dx */
+  int64_t x_group_stride, x_row_stride;     /* elements, >= 0 */
+  int64_t groups, rows, D;
+  const void* gain;                         /* NULL: 1, and gain_offset is not added */
+  const void* bias;
+  int gain_dtype;                           /* of gain, bias and their gradients */
+  int64_t gain_group_stride, bias_group_stride;
+  float gain_offset;
+  int center;                               /* 1 layer norm, 0 RMS norm */
+  double eps;
+  float* mean;                              /* center == 0: _fwd writes 0, _bwd does not read it */
+  float* rstd;
+};
+int unirl_layer_norm_fwd(const struct unirl_norm_desc* desc, void* y, void* stream);
+
+/* Bytes of scratch for unirl_layer_norm_bwd's dgain and dbias (the backward of the norm in front of
+ * unirl/models/qwen3/ar.py:82-99). */
+size_t unirl_layer_norm_bwd_scratch_bytes(int64_t groups, int64_t rows, int64_t D);
+
+/* Gradients of the same (unirl/models/qwen3/ar.py:82-99, unirl/models/sd3/diffusion.py:467-497 under
+ * autograd); desc->mean and ->rstd as the forward wrote them (mean only with center).  With
+ * a = dy (gain_offset + gain) and xh = (x - mu) s:
+ *     dx = s (a - xh mean(a xh) - mean(a))        (center == 0: without mean(a))
+ *     dgain = sum of dy xh, dbias = sum of dy, over the rows of the group (per_group != 0, [groups, D])
+ *             or over all rows ([D]); f32 sums in an order that depends on the shape alone
+ * dy: x's dtype, its own strides.  dx (dense), dgain, dbias may each be NULL; without rows dgain and
+ * dbias are zero.  scratch: device memory for dgain and dbias, not initialised, of at least
+ * unirl_layer_norm_bwd_scratch_bytes(); per_group: at most 65535 groups. */
+int unirl_layer_norm_bwd(const struct unirl_norm_desc* desc, const void* dy, int64_t dy_group_stride,
+                         int64_t dy_row_stride, void* dx, void* dgain, void* dbias, int per_group,
+                         void* scratch, size_t scratch_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Global norm of many gradients, sqrt(sum of squares over all of them): the grad norm of the
+ * optimizer step (unirl/train/fsdp_utils.py:313 sums the ranks' squares).  Squares are formed and
+ * added in fp64, in an order that depends on the sizes alone; Inf and NaN propagate.  `grads`,
+ * `numels` and `dtypes` are HOST arrays of n_tensors entries (at most 262144), each gradient dense;
+ * an empty list gives 0.  norm: one f32.
+ * ---------------------------------------------------------------------- */
+int unirl_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes,
+                    int64_t n_tensors, float* norm, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/* ------------------------------------------------------------------------
+ * One AdamW step over many tensors: the optimizer step that follows a policy's backward
+ * (unirl/train/stack.py:332).  With the gradient scaled by the clip factor c,
+ *     m = beta1 m + (1 - beta1) c g;   v = beta2 v + (1 - beta2) (c g)^2
+ *     p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * evaluated in f32 and stored in place; every tensor dense, element i of one lies at i in the others.
+ *
+ * state_bits 32: exp_avg, exp_avg_sq f32.  state_bits 8: one byte per element and one scale byte per
+ * 256 elements (the last block may be short): m = e4m3 (OCP, NaN 0x7f) * 2^(scale - 127), v = the
+ * half whose bits are byte << 7, * 2^(scale - 127); all bytes zero is a zero state.  They are rounded
+ * stochastically with a hash of (seed, t, index_base + i): the same call gives the same bytes,
+ * and a moving average that changes by less than a code step still moves by as much on average.
+ * A positive v is held as at least the least positive code.  An element that is not finite has the
+ * code of NaN (m) or of infinity or NaN (v) and does not enter its block's scale.
+ * index_base: a multiple of 256, which elements number i of the tensors add to it to be told apart.
+ *
+ * use_master: `master` f32 holds the parameters, the 16-bit `param` receives their rounded values.
+ * param_dtype any; grad_dtype the same or f32.
+ *
+ * The step's scalars are given in one of two ways:
+ *   control == NULL: step = t >= 1, lr, weight_decay, seed from the struct; c = 1, or with grad_norm
+ *       (device, f32) and max_norm >= 0: min(1, max_norm / (*grad_norm + 1e-6)).  skip_nonfinite:
+ *       nothing is written when *grad_norm is Inf or NaN.
+ *   control (device, UNIRL_ADAMW_CONTROL_BYTES): as unirl_adamw_advance left it on this stream; step,
+ *       lr, weight_decay, seed, grad_norm, max_norm and skip_nonfinite of the struct are not read.
+ * The tables travel in the kernel arguments: nothing is copied or kept, the arrays may be freed on
+ * return, and the call may be captured into a graph.
+ * ---------------------------------------------------------------------- */
+#define UNIRL_ADAMW_CONTROL_BYTES 32
+struct unirl_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* master;              /* use_master only */
+  uint8_t* exp_avg_scale;     /* state_bits 8 only: one per 256 elements */
+  uint8_t* exp_avg_sq_scale;
+  int64_t numel;
+  int64_t index_base;
+};
+struct unirl_adamw_params {
+  int param_dtype, grad_dtype; /* unirl_dtype */
+  int state_bits;              /* 8 or 32 */
+  int use_master;
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;                /* 1 for the first */
+  uint32_t seed;
+  const float* grad_norm;      /* device, or NULL */
+  float max_norm;              /* < 0: no clipping */
+  int skip_nonfinite;
+  const void* control;
+};
+int unirl_adamw_step(const struct unirl_adamw_tensor* tensors /* host */, int64_t n_tensors,
+                     const struct unirl_adamw_params* params /* host */, void* stream);
+
+/* The scalars of the next step, worked out on the device (a captured optimizer step, whose count and
+ * learning rate live there; unirl/train/stack.py:332): t = *step + 1; control receives what
+ * unirl_adamw_step reads; *step = t unless the step is skipped (skip_nonfinite and *grad_norm Inf or
+ * NaN).  lr_ptr (device f32) replaces lr when not NULL. */
+int unirl_adamw_advance(int64_t* step, void* control, double lr, const float* lr_ptr, double beta1,
+                        double beta2, double weight_decay, uint32_t seed, const float* grad_norm,
+                        float max_norm, int skip_nonfinite, void* stream);
+
+/* The values that 8-bit moments stand for, e.g. for a checkpoint of the optimizer that
+ * unirl/train/stack.py:332 steps: out_* [numel] of out_dtype, each may be NULL.  Both are exact in
+ * f32 and, but for values below its least normal number, in bf16. */
+int unirl_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const uint8_t* exp_avg_scale,
+                        const uint8_t* exp_avg_sq_scale, int64_t numel, void* out_exp_avg,
+                        void* out_exp_avg_sq, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -127,6 +127,70 @@ class SdeReplayDesc(Structure):
     ]
 
 
+class NormDesc(Structure):
+    """struct unirl_norm_desc."""
+
+    _fields_ = [
+        ("x", c_void_p),
+        ("dtype", c_int),
+        ("x_group_stride", c_int64),
+        ("x_row_stride", c_int64),
+        ("groups", c_int64),
+        ("rows", c_int64),
+        ("D", c_int64),
+        ("gain", c_void_p),
+        ("bias", c_void_p),
+        ("gain_dtype", c_int),
+        ("gain_group_stride", c_int64),
+        ("bias_group_stride", c_int64),
+        ("gain_offset", c_float),
+        ("center", c_int),
+        ("eps", c_double),
+        ("mean", c_void_p),
+        ("rstd", c_void_p),
+    ]
+
+
+class AdamwTensor(Structure):
+    """struct unirl_adamw_tensor."""
+
+    _fields_ = [
+        ("param", c_void_p),
+        ("grad", c_void_p),
+        ("exp_avg", c_void_p),
+        ("exp_avg_sq", c_void_p),
+        ("master", c_void_p),
+        ("exp_avg_scale", c_void_p),
+        ("exp_avg_sq_scale", c_void_p),
+        ("numel", c_int64),
+        ("index_base", c_int64),
+    ]
+
+
+class AdamwParams(Structure):
+    """struct unirl_adamw_params."""
+
+    _fields_ = [
+        ("param_dtype", c_int),
+        ("grad_dtype", c_int),
+        ("state_bits", c_int),
+        ("use_master", c_int),
+        ("lr", c_double),
+        ("beta1", c_double),
+        ("beta2", c_double),
+        ("eps", c_double),
+        ("weight_decay", c_double),
+        ("step", c_int64),
+        ("seed", ctypes.c_uint32),
+        ("grad_norm", c_void_p),
+        ("max_norm", c_float),
+        ("skip_nonfinite", c_int),
+        ("control", c_void_p),
+    ]
+
+
+ADAMW_CONTROL_BYTES = 32  # UNIRL_ADAMW_CONTROL_BYTES
+
 # enum unirl_dpm2_branch
 DPM2_DDIM, DPM2_FIRST, DPM2_SECOND = 0, 1, 2
 
@@ -246,6 +310,23 @@ _SIGNATURES = {
          c_void_p],
     ),
     "unirl_expand_groups": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p]),
+    "unirl_layer_norm_fwd": (c_int, [POINTER(NormDesc), c_void_p, c_void_p]),
+    "unirl_layer_norm_bwd_scratch_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "unirl_layer_norm_bwd": (
+        c_int,
+        [POINTER(NormDesc), c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p],
+    ),
+    "unirl_grad_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "unirl_adamw_step": (c_int, [c_void_p, c_int64, POINTER(AdamwParams), c_void_p]),
+    "unirl_adamw_advance": (
+        c_int,
+        [c_void_p, c_void_p, c_double, c_void_p, c_double, c_double, c_double, ctypes.c_uint32, c_void_p, c_float, c_int,
+         c_void_p],
+    ),
+    "unirl_adamw_moments": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p],
+    ),
     "unirl_gather_steps": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p],

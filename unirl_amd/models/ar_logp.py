@@ -24,6 +24,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import ops
+from .norm import layer_norm, rms_norm
 
 
 def _is_plain_linear(lm_head) -> bool:
@@ -251,6 +252,29 @@ def token_entropy(logits: torch.Tensor, temperature: float = 1.0) -> torch.Tenso
     return ent
 
 
+def _apply_final_norm(norm: Callable[[torch.Tensor], torch.Tensor], hidden: torch.Tensor) -> torch.Tensor:
+    """``norm(hidden)``; a plain ``nn.RMSNorm`` / ``nn.LayerNorm`` over the last dimension runs as one
+    fused kernel each way.  Subclasses, modules with hooks, other callables and autocast go through
+    their own call."""
+    from torch.nn.modules import module as _m
+
+    kind = type(norm)
+    own = (
+        kind in (torch.nn.RMSNorm, torch.nn.LayerNorm)
+        and not (norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks)
+        and not (_m._global_forward_hooks or _m._global_forward_pre_hooks or _m._global_backward_hooks
+                 or _m._global_backward_pre_hooks)
+        and tuple(norm.normalized_shape) == (hidden.shape[-1],) and hidden.shape[-1] <= ops.NORM_MAX_DIM
+        and hidden.is_cuda and hidden.dtype in _KERNEL_DTYPES and not torch.is_autocast_enabled("cuda")
+        and all(p.dtype in _KERNEL_DTYPES and p.device == hidden.device for p in norm.parameters())
+    )
+    if not own:
+        return norm(hidden)
+    if kind is torch.nn.LayerNorm:
+        return layer_norm(hidden, norm.weight, norm.bias, norm.eps)
+    return rms_norm(hidden, norm.weight, torch.finfo(hidden.dtype).eps if norm.eps is None else norm.eps)
+
+
 #: all of a replay's logits are kept for the backward (no second ``lm_head`` pass) up to this size
 KEEP_LOGITS_BYTES = 4 << 30
 #: replays of at least this many rows compute the hidden states' gradient on a transposed copy of the weight
@@ -266,6 +290,7 @@ def chunked_replay_logp(
     keep_logits: Optional[bool] = None,
     fused_head: Optional[bool] = None,
     transposed_head: Optional[bool] = None,
+    final_norm: Optional[Callable[[torch.Tensor], torch.Tensor]] = None,
 ) -> torch.Tensor:
     """Padded ``[B, T_max]`` fp32 log-probs of ``response_tokens`` under ``lm_head(resp_hidden)``.
 
@@ -307,10 +332,17 @@ def chunked_replay_logp(
     replays in any way -- an optimizer step, or a write through ``.data`` that no version counter
     records -- is always read afresh.  Left at ``None`` it is used for replays of at least
     ``TRANSPOSED_HEAD_MIN_ROWS`` rows.
+
+    ``final_norm`` is for hidden states taken before the model's last norm: it is applied to the
+    response's rows first.  An ``nn.RMSNorm`` or ``nn.LayerNorm`` over the hidden size runs as one fused
+    kernel forward and one backward (``models.rms_norm`` / ``layer_norm``: fp32 inside, one rounding),
+    any other callable as it is.
     """
     bsz, t_max = int(resp_hidden.size(0)), int(response_tokens.size(1))
     if t_max == 0:
         return resp_hidden.new_zeros((bsz, 0), dtype=torch.float32)
+    if final_norm is not None:
+        resp_hidden = _apply_final_norm(final_norm, resp_hidden[:, :t_max, :])
     if keep_logits is None:
         keep_logits = (
             _is_plain_linear(lm_head)

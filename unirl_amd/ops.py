@@ -7,6 +7,7 @@ API (``unirl_amd.sde``, ``unirl_amd.algorithms``, ...) is built on these.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import math
@@ -1495,6 +1496,414 @@ def expand_groups(unique: torch.Tensor, group_of: torch.Tensor, dtype: torch.dty
         )
     N.check(rc, "unirl_expand_groups")
     return out
+
+
+# ---------------------------------------------------------------------------
+# layer norm / RMS norm in front of a policy's output
+# ---------------------------------------------------------------------------
+NORM_MAX_DIM = 32768  # elements of a row
+
+
+def _norm_rows(x: torch.Tensor, per_group: bool) -> Tuple[torch.Tensor, int, int, int, int]:
+    """``(tensor, groups, rows, group stride, row stride)`` of ``x [..., D]``: read in place when its
+    leading dimensions are at most two runs of equally spaced rows (with ``per_group`` dimension 0 is
+    the groups), else from a contiguous copy.  Shared gains leave one partial sum per group, so many
+    short groups are copied together as well."""
+    D = x.shape[-1]
+    n = x.numel() // D if D else 0
+    if not x.is_contiguous():
+        runs: List[List[int]] = []  # [size, stride], outermost first; dimension 0 stays apart for groups
+        for i, (size, stride) in enumerate(zip(x.shape[:-1], x.stride()[:-1])):
+            if size == 1 and not (per_group and i == 0):
+                continue
+            if runs and not (per_group and len(runs) == 1) and runs[-1][1] == stride * size:
+                runs[-1] = [runs[-1][0] * size, stride]
+            else:
+                runs.append([size, stride])
+        if (x.stride(-1) == 1 or D == 1) and len(runs) <= 2 and (per_group or len(runs) < 2 or runs[0][0] <= 256):
+            while len(runs) < 2:
+                runs.insert(len(runs) if per_group else 0, [1, 0])
+            (G, gs), (R, rs) = runs
+            return x, G, R, gs, rs
+        x = x.contiguous()
+    if per_group:
+        G = x.shape[0]
+        R = n // G if G else 0
+        return x, G, R, R * D, D
+    return x, 1, n, 0, D
+
+
+def _norm_param(p: Optional[torch.Tensor], x: torch.Tensor, name: str) -> Tuple[Optional[torch.Tensor], bool]:
+    """A gain or bias with its elements adjacent, and whether it has one row per group."""
+    if p is None:
+        return None, False
+    N.require_device(p, name)
+    if p.device != x.device:
+        raise ValueError(f"{name} lives on {p.device}, x on {x.device}")
+    D = x.shape[-1]
+    if tuple(p.shape) != (D,) and not (p.dim() == 2 and x.dim() >= 2 and tuple(p.shape) == (x.shape[0], D)):
+        raise ValueError(f"{name} must be [{D}] or [{x.shape[0] if x.dim() > 1 else 'groups'}, {D}]; got {tuple(p.shape)}")
+    N.dtype_code(p.dtype)
+    return (p if p.stride(-1) == 1 or D <= 1 else p.contiguous()), p.dim() == 2
+
+
+def _norm_desc(x, weight, bias, eps, rms, unit_offset):
+    """``(desc, tensor read, per_group)`` with everything but the statistics filled in."""
+    N.require_device(x, "x")
+    code = N.dtype_code(x.dtype)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must be [..., D] with D >= 1; got {tuple(x.shape)}")
+    w, w_rows = _norm_param(weight, x, "weight")
+    b, b_rows = _norm_param(bias, x, "bias")
+    if w is not None and b is not None and (w.dtype != b.dtype or w_rows != b_rows):
+        raise ValueError(f"weight and bias differ: {w.dtype} {tuple(w.shape)}, {b.dtype} {tuple(b.shape)}")
+    per_group = w_rows or b_rows
+    t, G, R, gs, rs = _norm_rows(x, per_group)
+    p = w if w is not None else b
+    desc = N.NormDesc(
+        x=N.ptr(t), dtype=code, x_group_stride=gs, x_row_stride=rs, groups=G, rows=R, D=x.shape[-1], gain=N.ptr(w), bias=N.ptr(b),
+        gain_dtype=N.F32 if p is None else N.dtype_code(p.dtype),
+        gain_group_stride=w.stride(0) if w_rows else 0, bias_group_stride=b.stride(0) if b_rows else 0,
+        gain_offset=1.0 if unit_offset else 0.0, center=0 if rms else 1, eps=float(eps),
+    )
+    return desc, (t, w, b), per_group
+
+
+def layer_norm(
+    x: torch.Tensor,
+    weight: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    *,
+    eps: float = 1e-5,
+    rms: bool = False,
+    unit_offset: bool = False,
+    want_stats: bool = False,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """``(y, mean, rstd)`` of the layer norm of ``x [..., D]`` over its last dimension (``D <= 32768``);
+    ``rms``: root mean square instead of the centred one.  ``y = (x - mean) rstd weight + bias`` in
+    ``x``'s dtype, computed in fp32 and rounded once; ``unit_offset`` multiplies by ``1 + weight``.
+
+    ``weight`` / ``bias`` are ``[D]``, or ``[G, D]`` with one row for each ``x[g]`` (a modulated norm),
+    in one dtype of their own.  ``mean`` (``None`` for ``rms``) and ``rstd`` are fp32 ``x.shape[:-1]``,
+    only with ``want_stats``.  ``x`` may be a view whose rows are equally spaced (``hidden[:, a:b]``).
+    """
+    desc, held, _ = _norm_desc(x, weight, bias, eps, rms, unit_offset)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if want_stats:
+        rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        mean = None if rms else torch.empty_like(rstd)
+        desc.mean, desc.rstd = N.ptr(mean), N.ptr(rstd)
+    if y.numel():
+        with N.on_device(x.device):
+            rc = N.F.unirl_layer_norm_fwd(ctypes.byref(desc), N.ptr(y), N.current_stream(x.device))
+        N.check(rc, "unirl_layer_norm_fwd")
+    return y, mean, rstd
+
+
+def layer_norm_bwd(
+    dy: torch.Tensor,
+    x: torch.Tensor,
+    mean: Optional[torch.Tensor],
+    rstd: torch.Tensor,
+    weight: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    *,
+    rms: bool = False,
+    unit_offset: bool = False,
+    want_dx: bool = True,
+    want_dweight: bool = True,
+    want_dbias: bool = True,
+) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """``(dx, dweight, dbias)`` of :func:`layer_norm` for the gradient ``dy`` of ``y`` and the statistics
+    of ``want_stats``.  ``dx`` has ``x``'s dtype; the parameters' gradients have their shapes and dtype,
+    summed in fp32 over the rows that read them, in an order that depends on the shape alone.  ``bias``
+    gives its shape and dtype only; a gradient whose parameter is ``None`` is ``None``."""
+    desc, held, per_group = _norm_desc(x, weight, bias, 0.0, rms, unit_offset)
+    if dy.shape != x.shape:
+        raise ValueError(f"dy {tuple(dy.shape)} != x {tuple(x.shape)}")
+    if rstd.shape != x.shape[:-1] or (not rms and (mean is None or mean.shape != x.shape[:-1])):
+        raise ValueError("mean and rstd must be the statistics of this x")
+    device = x.device
+    rstd = N.as_operand(rstd, torch.float32, device)
+    mean = None if rms else N.as_operand(mean, torch.float32, device)
+    desc.mean, desc.rstd = N.ptr(mean), N.ptr(rstd)
+    g = dy if dy.dtype == x.dtype and dy.device == device else dy.detach().to(device=device, dtype=x.dtype)
+    g, G, R, gs, rs = _norm_rows(g, per_group)
+    if (G, R) != (desc.groups, desc.rows):  # the two are cut into groups unlike each other
+        g = g.contiguous()
+        R, G = desc.rows, desc.groups
+        gs, rs = R * desc.D, desc.D
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_dx else None
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=device) if want_dweight and weight is not None else None
+    db = torch.empty(bias.shape, dtype=bias.dtype, device=device) if want_dbias and bias is not None else None
+    if dx is None and dw is None and db is None:
+        return None, None, None
+    scratch = nbytes = None
+    if dw is not None or db is not None:
+        nbytes = int(N.F.unirl_layer_norm_bwd_scratch_bytes(desc.groups, desc.rows, desc.D))
+        scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    with N.on_device(device):
+        rc = N.F.unirl_layer_norm_bwd(
+            ctypes.byref(desc), N.ptr(g), gs, rs, N.ptr(dx) if dx is not None and dx.numel() else None, N.ptr(dw), N.ptr(db),
+            int(per_group), N.ptr(scratch), nbytes or 0, N.current_stream(device),
+        )
+    N.check(rc, "unirl_layer_norm_bwd")
+    return dx, dw, db
+
+
+# ---------------------------------------------------------------------------
+# the optimizer step: global gradient norm, AdamW
+# ---------------------------------------------------------------------------
+ADAMW_BLOCK = 256  # elements that share a scale of the 8-bit moments
+
+
+def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
+    """Global L2 norm of the tensors' elements together, as an fp32 0-dim tensor on their device.
+
+    fp32, bf16 and fp16 tensors may be mixed.  Squares are added in fp64 in an order that depends on
+    the sizes alone; Inf and NaN propagate.  Two launches for up to 160 tensors, one more for every
+    further 160; nothing is copied from the host and nothing synchronises.
+    """
+    ts = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    if not ts:
+        raise ValueError("grad_norm needs at least one tensor")
+    device = ts[0].device
+    N.require_device(ts[0], "grads[0]")
+    if any(t.device != device for t in ts):
+        raise ValueError("grad_norm: the tensors live on different devices")
+    n = len(ts)
+    ptrs = array.array("Q", [t.data_ptr() for t in ts])
+    numels = array.array("q", [t.numel() for t in ts])
+    codes = array.array("i", [N.dtype_code(t.dtype) for t in ts])
+    out = torch.empty((), dtype=torch.float32, device=device)
+    # scratch of this call alone: calls on other streams, and graphs, never share it
+    ws = torch.empty(int(N.F.unirl_workspace_bytes()), dtype=torch.uint8, device=device)
+    with N.on_device(device):
+        rc = N.F.unirl_grad_norm(
+            ptrs.buffer_info()[0], numels.buffer_info()[0], codes.buffer_info()[0], n, N.ptr(out), N.ptr(ws), ws.numel(),
+            N.current_stream(device),
+        )
+    N.check(rc, "unirl_grad_norm")
+    return out
+
+
+def _same_numel(name: str, tensors, numels, dtype, device) -> None:
+    for i, (t, n) in enumerate(zip(tensors, numels)):
+        if t.numel() != n or t.dtype != dtype or t.device != device or not t.is_contiguous():
+            raise ValueError(
+                f"{name}[{i}] must be a contiguous {dtype} tensor of {n} elements on {device}; got {t.dtype} "
+                f"{tuple(t.shape)} strides {t.stride()} on {t.device}"
+            )
+
+
+def _clip_args(grad_norm: Optional[torch.Tensor], max_norm: Optional[float], skip_nonfinite: bool, device) -> float:
+    if grad_norm is None:
+        if max_norm is not None or skip_nonfinite:
+            raise ValueError("max_norm and skip_nonfinite need grad_norm")
+        return -1.0
+    if grad_norm.numel() != 1 or grad_norm.dtype != torch.float32 or grad_norm.device != device:
+        raise ValueError(f"grad_norm must be one float32 value on {device}")
+    if max_norm is None:
+        return -1.0
+    if not float(max_norm) >= 0.0:
+        raise ValueError(f"max_norm must not be negative; got {max_norm}")
+    return float(max_norm)
+
+
+def _adamw_hyper(betas, eps: float, weight_decay: float) -> Tuple[float, float]:
+    b1, b2 = float(betas[0]), float(betas[1])
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+        raise ValueError(f"betas must lie in [0, 1); got {tuple(betas)}")
+    if not eps >= 0.0 or not weight_decay >= 0.0:
+        raise ValueError(f"eps and weight_decay must not be negative; got {eps}, {weight_decay}")
+    return b1, b2
+
+
+def adamw_step(
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor],
+    exp_avgs: Sequence[torch.Tensor],
+    exp_avg_sqs: Sequence[torch.Tensor],
+    *,
+    lr: Optional[float] = None,
+    betas: Tuple[float, float] = (0.9, 0.999),
+    eps: float = 1e-8,
+    weight_decay: float = 1e-2,
+    step: Optional[int] = None,
+    masters: Optional[Sequence[torch.Tensor]] = None,
+    exp_avg_scales: Optional[Sequence[torch.Tensor]] = None,
+    exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
+    index_bases: Optional[Sequence[int]] = None,
+    seed: int = 0,
+    grad_norm: Optional[torch.Tensor] = None,
+    max_norm: Optional[float] = None,
+    skip_nonfinite: bool = False,
+    control: Optional[torch.Tensor] = None,
+) -> None:
+    """One AdamW step (decoupled weight decay) over lists of tensors, in place, 48 tensors a launch::
+
+        m = b1 m + (1 - b1) c g;   v = b2 v + (1 - b2) (c g)^2
+        p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+
+    in fp32, each stored value rounded once.  ``c`` is 1, or with ``grad_norm`` (:func:`grad_norm`) and
+    ``max_norm`` the clip factor ``min(1, max_norm / (grad_norm + 1e-6))``, worked out on the device;
+    with ``skip_nonfinite`` nothing is written when the norm is Inf or NaN.
+
+    ``params`` share one dtype, ``grads`` the same one or fp32; all tensors are contiguous and must not
+    overlap.  ``masters`` (fp32) hold the values of 16-bit ``params``, which then receive the rounded
+    master.  The moments are fp32, or uint8 together with ``exp_avg_scales`` / ``exp_avg_sq_scales``
+    (uint8, one per 256 elements; zeros are the zero state): formats and stochastic rounding as in
+    :func:`adamw_moments`.  The rounding's random bits are a hash of ``(seed, step, index_bases[i] +
+    element)``; ``index_bases`` (multiples of 256) default to the tensors laid end to end.
+
+    ``step`` counts from 1.  A captured call repeats its ``step``, ``lr`` and ``seed`` in every replay; to
+    have them move, pass ``control`` from :func:`adamw_advance` instead of ``lr``, ``step``, ``weight_decay``,
+    ``seed``, ``grad_norm``, ``max_norm`` and ``skip_nonfinite``.
+    """
+    n = len(params)
+    states8 = exp_avg_scales is not None or exp_avg_sq_scales is not None
+    lists = {"grads": grads, "exp_avgs": exp_avgs, "exp_avg_sqs": exp_avg_sqs}
+    if masters is not None:
+        lists["masters"] = masters
+    if states8:
+        if exp_avg_scales is None or exp_avg_sq_scales is None:
+            raise ValueError("8-bit moments need exp_avg_scales and exp_avg_sq_scales")
+        lists.update(exp_avg_scales=exp_avg_scales, exp_avg_sq_scales=exp_avg_sq_scales)
+    if index_bases is not None:
+        lists["index_bases"] = index_bases
+    for name, items in lists.items():
+        if len(items) != n:
+            raise ValueError(f"{name} has {len(items)} entries for {n} params")
+    b1, b2 = _adamw_hyper(betas, eps, weight_decay)
+    if n == 0:
+        return
+    device, dtype = params[0].device, params[0].dtype
+    N.require_device(params[0], "params[0]")
+    code = N.dtype_code(dtype)
+    if control is not None:
+        if step is not None or lr is not None or grad_norm is not None or max_norm is not None or skip_nonfinite:
+            raise ValueError("control already holds lr, step and the clip factor: pass either those or control")
+        _same_numel("control", [control], [N.ADAMW_CONTROL_BYTES], torch.uint8, device)
+    elif lr is None or step is None or int(step) < 1:
+        raise ValueError(f"adamw_step needs lr and a step of at least 1 (or control); got lr={lr}, step={step}")
+    bound = _clip_args(grad_norm, max_norm, skip_nonfinite, device)
+    numels = [p.numel() for p in params]
+    _same_numel("params", params, numels, dtype, device)
+    gs = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    gdtype = gs[0].dtype
+    if gdtype != dtype and gdtype != torch.float32:
+        raise TypeError(f"gradients of {dtype} parameters must be {dtype} or float32; got {gdtype}")
+    _same_numel("grads", gs, numels, gdtype, device)
+    sdtype = torch.uint8 if states8 else torch.float32
+    _same_numel("exp_avgs", exp_avgs, numels, sdtype, device)
+    _same_numel("exp_avg_sqs", exp_avg_sqs, numels, sdtype, device)
+    if masters is not None:
+        if dtype == torch.float32:
+            raise ValueError("masters are for 16-bit params: fp32 params hold their own values")
+        _same_numel("masters", masters, numels, torch.float32, device)
+    zeros = [0] * n
+    scales = [zeros, zeros]
+    if states8:
+        blocks = [-(-k // ADAMW_BLOCK) for k in numels]
+        for name, items in (("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales)):
+            _same_numel(name, items, blocks, torch.uint8, device)
+        scales = [[t.data_ptr() for t in exp_avg_scales], [t.data_ptr() for t in exp_avg_sq_scales]]
+        if index_bases is None:
+            index_bases, at = [], 0
+            for k in blocks:
+                index_bases.append(at)
+                at += k * ADAMW_BLOCK
+    addresses = [p.data_ptr() for p in params]
+    if len(set(a for a, k in zip(addresses, numels) if k)) != n - numels.count(0):
+        raise ValueError("the same parameter appears more than once")
+    columns = (
+        addresses, [g.data_ptr() for g in gs], [t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs],
+        zeros if masters is None else [t.data_ptr() for t in masters], *scales, numels,
+        zeros if index_bases is None else index_bases,
+    )
+    table = array.array("q", [v for row in zip(*columns) for v in row])  # struct unirl_adamw_tensor[n]
+    q = N.AdamwParams(
+        param_dtype=code, grad_dtype=N.dtype_code(gdtype), state_bits=8 if states8 else 32, use_master=int(masters is not None),
+        lr=0.0 if lr is None else float(lr), beta1=b1, beta2=b2, eps=float(eps), weight_decay=float(weight_decay),
+        step=0 if step is None else int(step), seed=int(seed) & 0xFFFFFFFF, grad_norm=N.ptr(grad_norm), max_norm=bound,
+        skip_nonfinite=int(bool(skip_nonfinite)), control=N.ptr(control),
+    )
+    with N.on_device(device):
+        rc = N.F.unirl_adamw_step(table.buffer_info()[0], n, ctypes.byref(q), N.current_stream(device))
+    N.check(rc, "unirl_adamw_step")
+    # written behind autograd's back: whoever saved a parameter for a backward has to notice
+    torch.autograd.graph.increment_version(params)
+
+
+def adamw_advance(
+    step: torch.Tensor,
+    control: torch.Tensor,
+    *,
+    lr: Union[float, torch.Tensor],
+    betas: Tuple[float, float] = (0.9, 0.999),
+    weight_decay: float = 1e-2,
+    seed: int = 0,
+    grad_norm: Optional[torch.Tensor] = None,
+    max_norm: Optional[float] = None,
+    skip_nonfinite: bool = False,
+) -> None:
+    """The scalars of the next :func:`adamw_step`, worked out on the device: ``step`` (one int64, the
+    steps taken so far) goes up by one and ``control`` (uint8, 32 bytes) receives what ``adamw_step``
+    reads.  With ``skip_nonfinite`` and a norm that is Inf or NaN the count stays and that step writes
+    nothing.  ``lr`` may be an fp32 device scalar."""
+    N.require_device(step, "step")
+    device = step.device
+    if step.numel() != 1 or step.dtype != torch.int64:
+        raise ValueError(f"step must be one int64 value; got {step.dtype} {tuple(step.shape)}")
+    _same_numel("control", [control], [N.ADAMW_CONTROL_BYTES], torch.uint8, device)
+    b1, b2 = _adamw_hyper(betas, 0.0, weight_decay)
+    bound = _clip_args(grad_norm, max_norm, skip_nonfinite, device)
+    lr_ptr = None
+    if isinstance(lr, torch.Tensor):
+        if lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != device:
+            raise ValueError(f"a tensor lr must be one float32 value on {device}")
+        lr_ptr, lr = N.ptr(lr), 0.0
+    with N.on_device(device):
+        rc = N.F.unirl_adamw_advance(
+            N.ptr(step), N.ptr(control), float(lr), lr_ptr, b1, b2, float(weight_decay), int(seed) & 0xFFFFFFFF,
+            N.ptr(grad_norm), bound, int(bool(skip_nonfinite)), N.current_stream(device),
+        )
+    N.check(rc, "unirl_adamw_advance")
+
+
+def adamw_moments(
+    exp_avg: torch.Tensor,
+    exp_avg_sq: torch.Tensor,
+    exp_avg_scale: torch.Tensor,
+    exp_avg_sq_scale: torch.Tensor,
+    *,
+    dtype: torch.dtype = torch.float32,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(m, v)`` that 8-bit moments stand for, in ``dtype`` (exact in fp32; in bf16 but for values below
+    its least normal number).
+
+    ``m`` is an e4m3 value (sign, 4 exponent and 3 mantissa bits) and ``v`` the positive half whose bits
+    are ``byte << 7`` (5 exponent and 3 mantissa bits), each times ``2 ** (scale - 127)`` of its block of
+    256 elements.  The step rounds to them stochastically, so that their expectation is the exact
+    moving average; to nearest, an average that moves by 0.1 % a step would never leave its code.
+    """
+    N.require_device(exp_avg, "exp_avg")
+    device, n = exp_avg.device, exp_avg.numel()
+    blocks = -(-n // ADAMW_BLOCK)
+    _same_numel("exp_avg and exp_avg_sq", [exp_avg, exp_avg_sq], [n, n], torch.uint8, device)
+    _same_numel("exp_avg_scale and exp_avg_sq_scale", [exp_avg_scale, exp_avg_sq_scale], [blocks, blocks], torch.uint8, device)
+    code = N.dtype_code(dtype)
+    m = torch.empty(exp_avg.shape, dtype=dtype, device=device)
+    v = torch.empty(exp_avg_sq.shape, dtype=dtype, device=device)
+    if n:
+        with N.on_device(device):
+            rc = N.F.unirl_adamw_moments(
+                N.ptr(exp_avg), N.ptr(exp_avg_sq), N.ptr(exp_avg_scale), N.ptr(exp_avg_sq_scale), n, N.ptr(m), N.ptr(v), code,
+                N.current_stream(device),
+            )
+        N.check(rc, "unirl_adamw_moments")
+    return m, v
 
 
 METRIC_SLOTS: Dict[str, int] = {

@@ -1,0 +1,209 @@
+"""AdamW over all of a policy's parameters in a few launches.
+
+The optimizer step of the reference's train stack (``unirl/train/stack.py:332``): the gradients' global
+norm (``unirl/train/fsdp_utils.py:313``), the clip factor and the AdamW update.  The norm never leaves
+the device, and the clipped gradients are never written: the update multiplies by the factor as it
+reads them.
+"""
+
+from __future__ import annotations
+
+from typing import Any, Dict, List, Optional, Tuple
+
+import torch
+
+from .. import _native as N
+from .. import ops
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW``'s update (decoupled weight decay) with fused kernels.
+
+    ``state_bits``: moments in fp32 (32), or in one byte each with a power-of-two scale per 256
+    elements (8; formats in :func:`unirl_amd.ops.adamw_moments`).  ``master_weights`` keeps an fp32 copy of
+    16-bit parameters, without which updates below half a unit in the last place of a parameter are
+    lost.  Both may be set per parameter group.
+
+    ``max_grad_norm`` clips by the global norm of all groups' gradients; ``step()`` leaves that norm in
+    ``grad_norm`` (a device scalar; ``None`` without ``max_grad_norm`` and ``skip_nonfinite``).
+    ``skip_nonfinite`` makes a step whose norm is Inf or NaN write nothing and not count.
+
+    ``capturable`` keeps the count of steps on the device, one per group, so that ``step()`` can be
+    captured into a graph and replayed (``lr`` as an fp32 device scalar may then change between replays);
+    ``skip_nonfinite`` needs it.  The first step, which makes the state, has to run before the capture.
+    Otherwise each parameter counts the steps in which it had a gradient.
+
+    Parameters are contiguous fp32, bf16 or fp16 tensors on a HIP device; sparse gradients are refused.
+    """
+
+    def __init__(
+        self,
+        params,
+        lr=1e-3,
+        betas: Tuple[float, float] = (0.9, 0.999),
+        eps: float = 1e-8,
+        weight_decay: float = 1e-2,
+        *,
+        state_bits: int = 32,
+        master_weights: bool = False,
+        max_grad_norm: Optional[float] = None,
+        skip_nonfinite: bool = False,
+        capturable: bool = False,
+        seed: int = 0,
+    ) -> None:
+        if isinstance(lr, torch.Tensor):
+            if not capturable:
+                raise ValueError("a tensor lr needs capturable=True")
+        elif not lr >= 0.0:
+            raise ValueError(f"lr must not be negative; got {lr}")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"max_grad_norm must not be negative; got {max_grad_norm}")
+        if skip_nonfinite and not capturable:
+            raise ValueError("skip_nonfinite needs capturable=True: whether a step counts is known on the device only")
+        self.max_grad_norm = max_grad_norm
+        self.skip_nonfinite = bool(skip_nonfinite)
+        self.capturable = bool(capturable)
+        self.grad_norm: Optional[torch.Tensor] = None
+        self._next_base = 0
+        self._controls: Dict[int, torch.Tensor] = {}
+        defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                        master_weights=master_weights, seed=int(seed), step=None)
+        super().__init__(params, defaults)
+
+    def add_param_group(self, param_group: Dict[str, Any]) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        ops._adamw_hyper(group["betas"], group["eps"], group["weight_decay"])
+        if group["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32; got {group['state_bits']}")
+        for p in group["params"]:
+            N.dtype_code(p.dtype)
+            if not p.is_contiguous():
+                raise ValueError(f"parameters must be contiguous; got strides {p.stride()} of {tuple(p.shape)}")
+
+    # -- state -------------------------------------------------------------
+    def _new_state(self, group: Dict[str, Any], p: torch.Tensor) -> Dict[str, Any]:
+        N.require_device(p, "parameter")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: run one step before capturing: the state would be made anew by every replay")
+        blocks = -(-p.numel() // ops.ADAMW_BLOCK)
+        state: Dict[str, Any] = {"step": 0, "index_base": self._next_base}
+        self._next_base += blocks * ops.ADAMW_BLOCK
+        dtype = torch.float32 if group["state_bits"] == 32 else torch.uint8
+        for name in ("exp_avg", "exp_avg_sq"):
+            state[name] = torch.zeros(p.shape, dtype=dtype, device=p.device)
+            if dtype is torch.uint8:
+                state[name + "_scale"] = torch.zeros(blocks, dtype=torch.uint8, device=p.device)
+        if group["master_weights"] and p.dtype is not torch.float32:
+            state["master"] = p.detach().to(torch.float32, copy=True)
+        return state
+
+    def moments(self, p: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``(exp_avg, exp_avg_sq)`` of a parameter as fp32 values, whatever they are held in."""
+        s = self.state[p]
+        if "exp_avg_scale" not in s:
+            return s["exp_avg"], s["exp_avg_sq"]
+        return ops.adamw_moments(s["exp_avg"], s["exp_avg_sq"], s["exp_avg_scale"], s["exp_avg_sq_scale"])
+
+    def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
+        """State tensors keep the dtypes they were saved with (the base class casts them to the
+        parameter's)."""
+        ours = [p for g in self.param_groups for p in g["params"]]
+        bits = [g["state_bits"] for g in self.param_groups for _ in g["params"]]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        saved = state_dict["state"]
+        for p, b, i in zip(ours, bits, ids):
+            s = saved.get(i)
+            if s is None:
+                continue
+            dtype = torch.float32 if b == 32 else torch.uint8
+            if s["exp_avg"].dtype != dtype or s["exp_avg"].shape != p.shape:
+                raise ValueError(
+                    f"saved moments are {s['exp_avg'].dtype} {tuple(s['exp_avg'].shape)}; this optimizer holds {dtype} "
+                    f"{tuple(p.shape)}"
+                )
+        super().load_state_dict(state_dict)
+        self._controls.clear()
+        self._next_base = 0
+        for p, i in zip(ours, ids):
+            s = saved.get(i)
+            if s is None:
+                continue
+            self.state[p] = {k: v.detach().to(p.device, copy=True).contiguous() if isinstance(v, torch.Tensor) else v
+                             for k, v in s.items()}
+            end = s["index_base"] + -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
+            self._next_base = max(self._next_base, end)
+
+    # -- the step ------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        if capturing and not self.capturable:
+            raise RuntimeError("AdamW: a captured step needs capturable=True (the count of steps would not move)")
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is not None and p.grad.layout is not torch.strided:
+                    raise RuntimeError("AdamW does not support sparse gradients")
+        grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+        self.grad_norm = None
+        if grads and (self.max_grad_norm is not None or self.skip_nonfinite):
+            self.grad_norm = ops.grad_norm(grads)
+        clip = dict(grad_norm=self.grad_norm, max_norm=self.max_grad_norm, skip_nonfinite=self.skip_nonfinite)
+        if self.grad_norm is None:
+            clip = {}
+        for index, group in enumerate(self.param_groups):
+            with_grad = [p for p in group["params"] if p.grad is not None]
+            if not with_grad:
+                continue
+            for p in with_grad:
+                if not self.state[p]:
+                    self.state[p].update(self._new_state(group, p))
+            how: Dict[str, Any] = {}
+            if self.capturable:
+                how["control"] = self._advance(index, group, with_grad[0].device, clip)
+            else:
+                how.update(lr=float(group["lr"]), weight_decay=group["weight_decay"], seed=group["seed"], **clip)
+            buckets: Dict[Any, List[torch.Tensor]] = {}
+            for p in with_grad:
+                s = self.state[p]
+                if not self.capturable:
+                    s["step"] += 1
+                buckets.setdefault((p.dtype, p.grad.dtype, "master" in s, s["step"]), []).append(p)
+            for (_, _, master, count), ps in buckets.items():
+                states = [self.state[p] for p in ps]
+
+                def column(name):
+                    return [s[name] for s in states]
+
+                if not self.capturable:
+                    how["step"] = count
+                ops.adamw_step(
+                    ps, [p.grad for p in ps], column("exp_avg"), column("exp_avg_sq"), betas=group["betas"], eps=group["eps"],
+                    masters=column("master") if master else None,
+                    exp_avg_scales=column("exp_avg_scale") if group["state_bits"] == 8 else None,
+                    exp_avg_sq_scales=column("exp_avg_sq_scale") if group["state_bits"] == 8 else None,
+                    index_bases=column("index_base"), **how,
+                )
+        return loss
+
+    def _advance(self, index: int, group: Dict[str, Any], device: torch.device, clip: Dict[str, Any]) -> torch.Tensor:
+        """The group's count of steps goes up on the device; the step's scalars."""
+        count, control = group["step"], self._controls.get(index)
+        if count is None or control is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: run one step before capturing: the state would be made anew by every replay")
+            if count is None:
+                count = group["step"] = torch.zeros((), dtype=torch.int64, device=device)
+            elif count.device != device:
+                count = group["step"] = count.to(device)
+            control = self._controls[index] = torch.zeros(N.ADAMW_CONTROL_BYTES, dtype=torch.uint8, device=device)
+        ops.adamw_advance(count, control, lr=group["lr"], betas=group["betas"], weight_decay=group["weight_decay"],
+                          seed=group["seed"], **clip)
+        return control
+
+
+__all__ = ["AdamW"]
