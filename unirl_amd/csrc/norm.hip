@@ -18,10 +18,10 @@
 namespace unirl {
 
 constexpr int kNormMaxDim = 32768;
-constexpr int kNormRowsPerBlock = 4;       // one-wavefront rows: wavefronts of a workgroup
-constexpr int kNormTargetBlocks = 1024;    // backward: workgroups over all groups (4 a compute unit)
+constexpr int kNormFwdRows = 4;            // one-wavefront rows: wavefronts of a workgroup, forward
+constexpr int kNormBwdRows = 8;            // and backward, where fewer workgroups leave fewer partial rows
+constexpr int64_t kNormMaxBlocks = 1024;   // workgroups over all groups (4 a compute unit)
 constexpr int64_t kNormMaxGroups = 65535;  // of one launch (gridDim.y)
-constexpr int64_t kNormMaxBlocks = 1 << 21;  // forward: workgroups per group; the rest is looped over (a launch counts its threads in 32 bits)
 
 struct NormArgs {
   const void* x;
@@ -35,7 +35,7 @@ struct NormArgs {
   float gain_offset;
   int center;
   float eps, inv_d;
-  int D;
+  uint32_t D;
   int64_t rows;
   float* mean;
   float* rstd;
@@ -44,28 +44,119 @@ struct NormArgs {
   int64_t partial_bias;
 };
 
-// VEC elements of a gain or bias whose type is known at run time (wave-uniform), from the caches:
-// every row reads them.
-template <typename T, int VEC>
-__device__ __forceinline__ void cached_load(const T* p, float (&o)[VEC]) {
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) o[k] = Elem<T>::load(p + k);
+// Rows are read and written through buffer descriptors that end with the row: a lane behind the end
+// loads zeros and its stores are dropped, so no access stands behind a condition, and an address
+// is one 32-bit offset.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* row, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(row), 0, bytes, 0x00020000);
 }
-template <int VEC>
-__device__ __forceinline__ void load_param(const void* base, int dtype, int64_t at, float absent, float add, float (&o)[VEC]) {
+constexpr int kStreaming = 2;  // cache policy of data that is touched once
+
+// VEC consecutive elements of T as loaded (up to 16 bytes), and as floats.
+template <typename T, int VEC, int POLICY>
+struct Packed {
+  static constexpr int kBytes = VEC * (int)sizeof(T);
+  static constexpr int kWords = (kBytes + 3) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    if constexpr (kBytes == 32) {
+      const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, POLICY);
+      const u32x4 b = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, 0, POLICY);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = a[k], w[4 + k] = b[k];
+    } else if constexpr (kBytes == 16) {
+      const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, POLICY);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = a[k];
+    } else if constexpr (kBytes == 8) {
+      const u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, POLICY);
+      w[0] = a[0];
+      w[1] = a[1];
+    } else if constexpr (kBytes == 4) {
+      w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, POLICY);
+    } else {
+      w[0] = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, POLICY);
+    }
+  }
+  __device__ __forceinline__ float get(int k) const {
+    if constexpr (sizeof(T) == 4)
+      return __uint_as_float(w[k]);
+    else if constexpr (std::is_same<T, bf16_t>::value)
+      return __uint_as_float(k & 1 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16);
+    else
+      return f16_bits_to_f32(k & 1 ? w[k / 2] >> 16 : w[k / 2] & 0xffffu);
+  }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(__amdgpu_buffer_rsrc_t r, uint32_t off, const float (&o)[VEC]) {
+  if constexpr (VEC == 1) {
+    if constexpr (sizeof(T) == 4) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[0]), r, off, 0, kStreaming);
+    } else {
+      T t;
+      Elem<T>::store(&t, o[0]);
+      __builtin_amdgcn_raw_buffer_store_b16((short)t.bits, r, off, 0, kStreaming);
+    }
+  } else {
+    u32x4 v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(T) == 4)
+        v[k] = __float_as_uint(o[k]);
+      else if constexpr (std::is_same<T, bf16_t>::value)
+        v[k] = f32x2_to_bf16x2_bits(o[2 * k], o[2 * k + 1]);
+      else
+        v[k] = f32_to_f16_bits(o[2 * k]) | (f32_to_f16_bits(o[2 * k + 1]) << 16);
+    }
+    __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, kStreaming);
+  }
+}
+
+// One lane's share of a row: E elements in vectors `step` elements apart.
+template <typename T, int VEC, int E>
+struct RowRegs {
+  Packed<T, VEC, kStreaming> q[E / VEC];
+  __device__ __forceinline__ void load(const T* row, uint32_t D, uint32_t col, uint32_t step) {
+    const __amdgpu_buffer_rsrc_t r = row_rsrc(row, D * (uint32_t)sizeof(T));
+#pragma unroll
+    for (int j = 0; j < E / VEC; ++j) q[j].load(r, (col + j * step) * (uint32_t)sizeof(T));
+  }
+  __device__ __forceinline__ void unpack(float (&v)[E]) const {
+#pragma unroll
+    for (int j = 0; j < E / VEC; ++j)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[j * VEC + k] = q[j].get(k);
+  }
+};
+
+// A lane's share of a gain or bias (from the caches: every row reads it), all loads in flight at once.
+template <typename W, int VEC, int E>
+__device__ __forceinline__ void load_param_as(const void* base, int64_t at, uint32_t D, uint32_t col, uint32_t step, float (&o)[E]) {
+  const __amdgpu_buffer_rsrc_t r = row_rsrc((const W*)base + at, D * (uint32_t)sizeof(W));
+  Packed<W, VEC, 0> q[E / VEC];
+#pragma unroll
+  for (int j = 0; j < E / VEC; ++j) q[j].load(r, (col + j * step) * (uint32_t)sizeof(W));
+#pragma unroll
+  for (int j = 0; j < E / VEC; ++j)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) o[j * VEC + k] = q[j].get(k);
+}
+template <int VEC, int E>
+__device__ __forceinline__ void load_param(const void* base, int dtype, int64_t at, uint32_t D, uint32_t col, uint32_t step,
+                                           float absent, float add, float (&o)[E]) {
   if (!base) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) o[k] = absent;
+    for (int k = 0; k < E; ++k) o[k] = absent;
     return;
   }
   if (dtype == UNIRL_F32)
-    cached_load<float, VEC>((const float*)base + at, o);
+    load_param_as<float, VEC, E>(base, at, D, col, step, o);
   else if (dtype == UNIRL_BF16)
-    cached_load<bf16_t, VEC>((const bf16_t*)base + at, o);
+    load_param_as<bf16_t, VEC, E>(base, at, D, col, step, o);
   else
-    cached_load<f16_t, VEC>((const f16_t*)base + at, o);
+    load_param_as<f16_t, VEC, E>(base, at, D, col, step, o);
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) o[k] += add;
+  for (int k = 0; k < E; ++k) o[k] += add;
 }
 
 // Sum over the row's threads, in every one of them.
@@ -77,125 +168,109 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
     return block_sum(v, lds);
 }
 
-template <typename T, int VEC, int E, bool ONE_WAVE>
-__device__ __forceinline__ void norm_fwd_row(const NormArgs& A, int64_t row, int tid, int nthreads, float* lds) {
-  const int64_t group = blockIdx.y;
-  const T* x = (const T*)A.x + group * A.x_group_stride + row * A.x_row_stride;
-  const int64_t flat = group * A.rows + row;
-  T* y = (T*)A.out + flat * A.D;
-  int cols[E / VEC];
-  float v[E];
-#pragma unroll
-  for (int j = 0; j < E / VEC; ++j) {
-    cols[j] = (j * nthreads + tid) * VEC;
-    float t[VEC];
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) t[k] = 0.0f;
-    if (cols[j] < A.D) Vec<T, VEC>::load(x + cols[j], t);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) v[j * VEC + k] = t[k];
-  }
-  float mean = 0.0f;
-  if (A.center) {
-    float s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < E; ++k) s += v[k];
-    mean = row_sum<ONE_WAVE>(s, lds) * A.inv_d;
-#pragma unroll
-    for (int j = 0; j < E / VEC; ++j)
-      if (cols[j] < A.D)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[j * VEC + k] -= mean;
-  }
-  float q = 0.0f;
-#pragma unroll
-  for (int k = 0; k < E; ++k) q = fmaf(v[k], v[k], q);
-  const float rstd = 1.0f / sqrtf(row_sum<ONE_WAVE>(q, lds) * A.inv_d + A.eps);
-#pragma unroll
-  for (int j = 0; j < E / VEC; ++j) {
-    if (cols[j] >= A.D) continue;
-    float o[VEC], w[VEC], b[VEC];
-    load_param<VEC>(A.gain, A.gain_dtype, group * A.gain_group_stride + cols[j], 1.0f, A.gain_offset, w);
-    load_param<VEC>(A.bias, A.gain_dtype, group * A.bias_group_stride + cols[j], 0.0f, 0.0f, b);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) o[k] = fmaf(v[j * VEC + k] * rstd, w[k], b[k]);
-    Vec<T, VEC>::store(y + cols[j], o);
-  }
-  if (tid == 0) {
-    if (A.mean) A.mean[flat] = mean;
-    if (A.rstd) A.rstd[flat] = rstd;
-  }
-}
-
-template <typename T, int VEC, int E, bool ONE_WAVE>
-__global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void norm_fwd_kernel(NormArgs A) {
-  __shared__ float lds[16];
-  const int tid = ONE_WAVE ? threadIdx.x & (kWave - 1) : threadIdx.x;
-  const int nthreads = ONE_WAVE ? kWave : blockDim.x;
-  const int64_t first = ONE_WAVE ? (int64_t)blockIdx.x * kNormRowsPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)
-                                 : (int64_t)blockIdx.x;
-  const int64_t stride = ONE_WAVE ? (int64_t)gridDim.x * kNormRowsPerBlock : (int64_t)gridDim.x;
-  for (int64_t row = first; row < A.rows; row += stride) norm_fwd_row<T, VEC, E, ONE_WAVE>(A, row, tid, nthreads, lds);
-}
-
-// Each wavefront (or workgroup) walks over rows of one group and keeps the sums of its columns in
-// registers; a workgroup leaves one partial row per sum, and norm_param_kernel adds those in order.
+// Both kernels: a wavefront (or workgroup) walks over rows of one group with the gain in registers and
+// the next row on its way while it works on one.
 template <typename T, int VEC, int E, bool ONE_WAVE, bool BIAS>
-__global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void norm_bwd_kernel(NormArgs A) {
-  extern __shared__ float sums[];  // ONE_WAVE: D floats to join the wavefronts; else 2 x 2 x 16 floats
-  const int tid = ONE_WAVE ? threadIdx.x & (kWave - 1) : threadIdx.x;
-  const int nthreads = ONE_WAVE ? kWave : blockDim.x;
+__global__ __launch_bounds__(ONE_WAVE ? kNormFwdRows * kWave : 1024) void norm_fwd_kernel(NormArgs A) {
+  __shared__ float lds[16];
+  const uint32_t tid = ONE_WAVE ? threadIdx.x & (kWave - 1) : threadIdx.x;
+  const uint32_t step = (ONE_WAVE ? kWave : blockDim.x) * VEC;
+  const uint32_t col = tid * VEC;
+  const int64_t first = ONE_WAVE ? (int64_t)blockIdx.x * kNormFwdRows + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)
+                                 : (int64_t)blockIdx.x;
+  const int64_t stride = ONE_WAVE ? (int64_t)gridDim.x * kNormFwdRows : (int64_t)gridDim.x;
+  if (first >= A.rows) return;
+  const int64_t group = blockIdx.y;
+  const T* x = (const T*)A.x + group * A.x_group_stride;
+  RowRegs<T, VEC, E> raw;
+  raw.load(x + first * A.x_row_stride, A.D, col, step);
+  float w[E], b[BIAS ? E : 1];
+  load_param<VEC, E>(A.gain, A.gain_dtype, group * A.gain_group_stride, A.D, col, step, 1.0f, A.gain_offset, w);
+  if constexpr (BIAS) load_param<VEC, E>(A.bias, A.gain_dtype, group * A.bias_group_stride, A.D, col, step, 0.0f, 0.0f, b);
+
+  for (int64_t row = first; row < A.rows; row += stride) {
+    float v[E];
+    raw.unpack(v);
+    if (row + stride < A.rows) raw.load(x + (row + stride) * A.x_row_stride, A.D, col, step);
+    float mean = 0.0f;
+    if (A.center) {
+      float s = 0.0f;
+#pragma unroll
+      for (int k = 0; k < E; ++k) s += v[k];
+      mean = row_sum<ONE_WAVE>(s, lds) * A.inv_d;
+#pragma unroll
+      for (int j = 0; j < E / VEC; ++j)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[j * VEC + k] = col + j * step < A.D ? v[j * VEC + k] - mean : 0.0f;
+    }
+    float q = 0.0f;
+#pragma unroll
+    for (int k = 0; k < E; ++k) q = fmaf(v[k], v[k], q);
+    const float rstd = 1.0f / sqrtf(row_sum<ONE_WAVE>(q, lds) * A.inv_d + A.eps);
+    const int64_t flat = group * A.rows + row;
+    const __amdgpu_buffer_rsrc_t y = row_rsrc((T*)A.out + flat * A.D, A.D * (uint32_t)sizeof(T));
+#pragma unroll
+    for (int j = 0; j < E / VEC; ++j) {
+      float o[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float xh = v[j * VEC + k] * rstd;
+        o[k] = BIAS ? fmaf(xh, w[j * VEC + k], b[BIAS ? j * VEC + k : 0]) : xh * w[j * VEC + k];
+      }
+      store_vec<T, VEC>(y, (col + j * step) * (uint32_t)sizeof(T), o);
+    }
+    if (tid == 0) {
+      if (A.mean) A.mean[flat] = mean;
+      if (A.rstd) A.rstd[flat] = rstd;
+    }
+  }
+}
+
+// The sums of the columns stay in registers as well; a workgroup leaves one partial row per sum, and
+// norm_param_kernel adds those in order.
+template <typename T, int VEC, int E, bool ONE_WAVE, bool BIAS>
+__global__ __launch_bounds__(ONE_WAVE ? kNormBwdRows * kWave : 1024) void norm_bwd_kernel(NormArgs A) {
+  extern __shared__ float sums[];  // ONE_WAVE: 4 D floats to join the wavefronts; else 2 x 2 x 16 floats
+  const uint32_t tid = ONE_WAVE ? threadIdx.x & (kWave - 1) : threadIdx.x;
+  const uint32_t step = (ONE_WAVE ? kWave : blockDim.x) * VEC;
+  const uint32_t col = tid * VEC;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t group = blockIdx.y;
   const T* x = (const T*)A.x + group * A.x_group_stride;
   const T* dy = (const T*)A.dy + group * A.dy_group_stride;
-
-  int cols[E / VEC];
-#pragma unroll
-  for (int j = 0; j < E / VEC; ++j) cols[j] = (j * nthreads + tid) * VEC;
-  float w[E];
-#pragma unroll
-  for (int j = 0; j < E / VEC; ++j) {
-    float t[VEC];
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) t[k] = 0.0f;
-    if (cols[j] < A.D)
-      load_param<VEC>(A.gain, A.gain_dtype, group * A.gain_group_stride + cols[j], 1.0f, A.gain_offset, t);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) w[j * VEC + k] = t[k];
+  const int64_t first = ONE_WAVE ? (int64_t)blockIdx.x * kNormBwdRows + wave : (int64_t)blockIdx.x;
+  const int64_t stride = ONE_WAVE ? (int64_t)gridDim.x * kNormBwdRows : (int64_t)gridDim.x;
+  RowRegs<T, VEC, E> rx, rg;
+  float rstd = 0.0f, mean = 0.0f;
+  if (first < A.rows) {
+    rx.load(x + first * A.x_row_stride, A.D, col, step);
+    rg.load(dy + first * A.dy_row_stride, A.D, col, step);
   }
-  float dw[E], db[E];
+  float w[E];
+  load_param<VEC, E>(A.gain, A.gain_dtype, group * A.gain_group_stride, A.D, col, step, 1.0f, A.gain_offset, w);
+  float dw[E], db[BIAS ? E : 1];
 #pragma unroll
-  for (int k = 0; k < E; ++k) dw[k] = db[k] = 0.0f;
+  for (int k = 0; k < E; ++k) dw[k] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < (BIAS ? E : 1); ++k) db[k] = 0.0f;
 
-  const int64_t first = ONE_WAVE ? (int64_t)blockIdx.x * kNormRowsPerBlock + wave : (int64_t)blockIdx.x;
-  const int64_t stride = ONE_WAVE ? (int64_t)gridDim.x * kNormRowsPerBlock : (int64_t)gridDim.x;
   int parity = 0;
   for (int64_t row = first; row < A.rows; row += stride) {
     const int64_t flat = group * A.rows + row;
-    const float rstd = A.rstd[flat];
-    const float mean = A.center ? A.mean[flat] : 0.0f;
+    rstd = A.rstd[flat];
+    if (A.center) mean = A.mean[flat];
     float xh[E], g[E];
-#pragma unroll
-    for (int j = 0; j < E / VEC; ++j) {
-      float tx[VEC], tg[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) tx[k] = tg[k] = 0.0f;
-      if (cols[j] < A.D) {
-        Vec<T, VEC>::load(x + row * A.x_row_stride + cols[j], tx);
-        Vec<T, VEC>::load(dy + row * A.dy_row_stride + cols[j], tg);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) tx[k] = (tx[k] - mean) * rstd;
-      }
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        xh[j * VEC + k] = tx[k];
-        g[j * VEC + k] = tg[k];
-      }
+    rx.unpack(xh);
+    rg.unpack(g);
+    if (row + stride < A.rows) {
+      rx.load(x + (row + stride) * A.x_row_stride, A.D, col, step);
+      rg.load(dy + (row + stride) * A.dy_row_stride, A.D, col, step);
     }
+    // behind the row's end dy is 0, and with it every product below
     float c1 = 0.0f, c2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < E; ++k) {
+      xh[k] = (xh[k] - mean) * rstd;
       dw[k] = fmaf(g[k], xh[k], dw[k]);
       if constexpr (BIAS) db[k] += g[k];
       g[k] *= w[k];
@@ -227,14 +302,13 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void norm_bwd_kernel(NormArg
     c1 *= A.inv_d;
     c2 *= A.inv_d;
     if (A.out) {
-      T* dx = (T*)A.out + flat * A.D;
+      const __amdgpu_buffer_rsrc_t dx = row_rsrc((T*)A.out + flat * A.D, A.D * (uint32_t)sizeof(T));
 #pragma unroll
       for (int j = 0; j < E / VEC; ++j) {
-        if (cols[j] >= A.D) continue;
         float o[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o[k] = (fmaf(-xh[j * VEC + k], c1, g[j * VEC + k]) - c2) * rstd;
-        Vec<T, VEC>::store(dx + cols[j], o);
+        store_vec<T, VEC>(dx, (col + j * step) * (uint32_t)sizeof(T), o);
       }
     }
   }
@@ -242,51 +316,75 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void norm_bwd_kernel(NormArg
 
 #pragma unroll
   for (int which = 0; which < (BIAS ? 2 : 1); ++which) {
-    float(&acc)[E] = which ? db : dw;
     float* out = A.partial + (which ? A.partial_bias : 0) + (group * gridDim.x + blockIdx.x) * A.D;
+    float acc[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) acc[k] = which ? db[BIAS ? k : 0] : dw[k];
     if constexpr (ONE_WAVE) {
-      // the wavefronts add their sums in order
-      for (int turn = 0; turn < kNormRowsPerBlock; ++turn) {
-        __syncthreads();
-        if (wave != turn) continue;
+      // the second half of the wavefronts leaves its sums in LDS, the first adds its own, then every
+      // thread adds the four sums of its columns
+      constexpr int kHalf = kNormBwdRows / 2;
+      float* mine = sums + (wave % kHalf) * A.D;
+      if (which) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < E / VEC; ++j) {
-          if (cols[j] >= A.D) continue;
+      for (int pass = 0; pass < 2; ++pass) {
+        if (wave / kHalf != pass) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            const float v = turn ? sums[cols[j] + k] + acc[j * VEC + k] : acc[j * VEC + k];
-            if (turn == kNormRowsPerBlock - 1)
-              out[cols[j] + k] = v;
-            else
-              sums[cols[j] + k] = v;
+          for (int j = 0; j < E / VEC; ++j) {
+            if (col + j * step >= A.D) continue;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+              const uint32_t c = col + j * step + k;
+              mine[c] = pass ? mine[c] + acc[j * VEC + k] : acc[j * VEC + k];
+            }
           }
         }
+        __syncthreads();
+      }
+      for (uint32_t c = threadIdx.x; c < A.D; c += kNormBwdRows * kWave) {
+        float v = sums[c];
+#pragma unroll
+        for (int h = 1; h < kHalf; ++h) v += sums[h * A.D + c];
+        out[c] = v;
       }
     } else {
 #pragma unroll
       for (int j = 0; j < E / VEC; ++j) {
-        if (cols[j] >= A.D) continue;
+        if (col + j * step >= A.D) continue;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) out[cols[j] + k] = acc[j * VEC + k];
+        for (int k = 0; k < VEC; ++k) out[col + j * step + k] = acc[j * VEC + k];
       }
     }
   }
 }
 
-// out[set][c] = sum of `n` partial rows, in a fixed order: 16 columns x 16 slices of the rows a workgroup.
+// out[set][c] = sum of `n` partial rows, in a fixed order: 32 columns x 32 slices of the rows a
+// workgroup, eight rows' loads of a lane in flight (a plain loop makes one trip to memory per row).
+// blockIdx.z: dgain, dbias.
 template <typename O>
-__global__ __launch_bounds__(256) void norm_param_kernel(const float* partial, int64_t n, int D, O* out) {
-  __shared__ float lds[256];
-  const int c = threadIdx.x & 15, slice = threadIdx.x >> 4;
-  const int64_t col = (int64_t)blockIdx.x * 16 + c;
-  const float* p = partial + (int64_t)blockIdx.y * n * D;
+__global__ __launch_bounds__(1024) void norm_param_kernel(const float* partial, int64_t partial_bias, int64_t n, uint32_t D, O* dgain,
+                                                         O* dbias) {
+  __shared__ float lds[32][33];
+  O* out = blockIdx.z ? dbias : dgain;
+  if (!out) return;
+  const int c = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const uint32_t col = blockIdx.x * 32 + c;
+  const float* p = partial + (blockIdx.z ? partial_bias : 0) + (int64_t)blockIdx.y * n * D + (col < D ? col : D - 1);
   float s = 0.0f;
-  if (col < D)
-    for (int64_t i = slice; i < n; i += 16) s += p[i * D + col];
-  lds[threadIdx.x] = s;
+  for (int64_t i0 = slice; i0 < n; i0 += 32 * 8) {
+    float t[8];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const int64_t i = i0 + 32 * b;
+      t[b] = p[(i < n ? i : n - 1) * D];
+    }
+#pragma unroll
+    for (int b = 0; b < 8; ++b) s += i0 + 32 * b < n ? t[b] : 0.0f;
+  }
+  lds[slice][c] = s;
   __syncthreads();
   if (slice == 0 && col < D) {
-    for (int k = 1; k < 16; ++k) s += lds[k * 16 + c];
+    for (int k = 1; k < 32; ++k) s += lds[k][c];
     Elem<O>::store(out + (int64_t)blockIdx.y * D + col, s);
   }
 }
@@ -296,58 +394,84 @@ struct NormShape {
   bool one_wave;
   int vec, elems, threads;
 };
-// A lane holds 8, 16 or 32 elements of a row.  Rows of up to 64 * 32 elements belong to one wavefront
-// (no barrier), longer ones to a workgroup of as many threads as 8 elements each ask for, up to 1024.
-static NormShape norm_shape(int64_t D, int dtype, bool vectors) {
+// Rows of up to 64 * 64 elements (forward) or 64 * 40 (backward, whose lanes hold five numbers per
+// element) belong to one wavefront (no barrier), longer ones to a workgroup of as many threads as
+// 8 elements each ask for, up to 1024.
+static NormShape norm_shape(int64_t D, int dtype, bool vectors, bool backward) {
   NormShape S;
   S.vec = vectors ? 16 / (int)dtype_size(dtype) : 1;
-  S.one_wave = D <= kWave * 32;
+  S.one_wave = D <= kWave * (vectors ? (backward ? 40 : 64) : 32);
   if (S.one_wave) {
-    S.elems = D <= kWave * 8 ? 8 : (D <= kWave * 16 ? 16 : 32);
-    S.threads = kWave * kNormRowsPerBlock;
+    const int need = (int)((D + kWave - 1) / kWave);  // elements of a lane
+    S.elems = need <= 8 ? 8 : (need <= 16 ? 16 : (need <= 32 && !vectors ? 32 : (need + 7) / 8 * 8));
+    if (S.elems == 56) S.elems = 64;
+    S.threads = kWave * (backward ? kNormBwdRows : kNormFwdRows);
   } else {
     S.elems = D <= 1024 * 8 ? 8 : (D <= 1024 * 16 ? 16 : 32);
     S.threads = (int)((D + S.elems * kWave - 1) / (S.elems * kWave)) * kWave;
   }
   return S;
 }
-static int64_t norm_bwd_blocks(int64_t groups, int64_t rows, bool one_wave) {
-  const int64_t most = one_wave ? (rows + kNormRowsPerBlock - 1) / kNormRowsPerBlock : rows;
-  const int64_t want = (kNormTargetBlocks + groups - 1) / groups;
+// Workgroups of one group.  Forward: up to 4 a compute unit.  Backward: as many as stay resident (16
+// wavefronts a compute unit for the narrower rows, 8 for those whose lanes need most of the registers)
+// with two rows a wavefront at least, since each leaves a partial row of D sums.
+static int64_t norm_blocks(const NormShape& S, int64_t groups, int64_t rows, bool backward) {
+  const int64_t rows_at_once = S.one_wave ? S.threads / kWave : 1;
+  const int64_t most = (rows + rows_at_once - 1) / rows_at_once;
+  int64_t total = kNormMaxBlocks;
+  if (backward) {
+    total = S.elems <= 16 ? 4096 : 2048;
+    total = total / (S.threads / kWave);
+    if (total < 256) total = 256;
+    const int64_t enough = (rows * groups + 2 * rows_at_once - 1) / (2 * rows_at_once);
+    if (total > enough) total = enough;
+  }
+  const int64_t want = (total + groups - 1) / groups;
   return want < most ? want : most;
 }
 
+template <typename T, int VEC, int E, bool ONE_WAVE, bool BIAS>
+static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool backward, hipStream_t s) {
+  if (!backward) {
+    hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, ONE_WAVE, BIAS>), grid, dim3(S.threads), 0, s, A);
+  } else if constexpr (!ONE_WAVE || E <= 40) {
+    hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, ONE_WAVE, BIAS>), grid, dim3(S.threads),
+                       ONE_WAVE ? (size_t)A.D * (kNormBwdRows / 2 * 4) : 64 * 4, s, A);
+  }
+}
 template <typename T, int VEC, int E>
 static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool backward, bool bias, hipStream_t s) {
-  const dim3 block(S.threads);
-  if (!backward) {
-    if (S.one_wave)
-      hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, true>), grid, block, 0, s, A);
+  if (S.one_wave) {
+    if (bias)
+      launch_norm<T, VEC, E, true, true>(A, S, grid, backward, s);
     else
-      hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, false>), grid, block, 0, s, A);
-    return;
+      launch_norm<T, VEC, E, true, false>(A, S, grid, backward, s);
+  } else if constexpr (E == 8 || E == 16 || E == 32) {
+    if (bias)
+      launch_norm<T, VEC, E, false, true>(A, S, grid, backward, s);
+    else
+      launch_norm<T, VEC, E, false, false>(A, S, grid, backward, s);
   }
-  const size_t lds = S.one_wave ? (size_t)A.D * 4 : 64 * 4;
-  if (S.one_wave && bias)
-    hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, true, true>), grid, block, lds, s, A);
-  else if (S.one_wave)
-    hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, true, false>), grid, block, lds, s, A);
-  else if (bias)
-    hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, true>), grid, block, lds, s, A);
-  else
-    hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, false>), grid, block, lds, s, A);
 }
 template <typename T>
 static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool backward, bool bias, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
   if (S.vec == 1) {
-    if (S.elems == 8) return launch_norm<T, 1, 8>(A, S, grid, backward, bias, s);
-    if (S.elems == 16) return launch_norm<T, 1, 16>(A, S, grid, backward, bias, s);
-    return launch_norm<T, 1, 32>(A, S, grid, backward, bias, s);
+    switch (S.elems) {
+      case 8: return launch_norm<T, 1, 8>(A, S, grid, backward, bias, s);
+      case 16: return launch_norm<T, 1, 16>(A, S, grid, backward, bias, s);
+      default: return launch_norm<T, 1, 32>(A, S, grid, backward, bias, s);
+    }
   }
-  if (S.elems == 8) return launch_norm<T, V, 8>(A, S, grid, backward, bias, s);
-  if (S.elems == 16) return launch_norm<T, V, 16>(A, S, grid, backward, bias, s);
-  return launch_norm<T, V, 32>(A, S, grid, backward, bias, s);
+  switch (S.elems) {
+    case 8: return launch_norm<T, V, 8>(A, S, grid, backward, bias, s);
+    case 16: return launch_norm<T, V, 16>(A, S, grid, backward, bias, s);
+    case 24: return launch_norm<T, V, 24>(A, S, grid, backward, bias, s);
+    case 32: return launch_norm<T, V, 32>(A, S, grid, backward, bias, s);
+    case 40: return launch_norm<T, V, 40>(A, S, grid, backward, bias, s);
+    case 48: return launch_norm<T, V, 48>(A, S, grid, backward, bias, s);
+    default: return launch_norm<T, V, 64>(A, S, grid, backward, bias, s);
+  }
 }
 static void launch_norm(const NormArgs& A, const NormShape& S, int dtype, dim3 grid, bool backward, bool bias,
                         hipStream_t s) {
@@ -363,6 +487,13 @@ static void launch_norm(const NormArgs& A, const NormShape& S, int dtype, dim3 g
 static bool vectors_ok(const void* p, int64_t gs, int64_t rs, int64_t D, int64_t groups, int64_t rows, size_t esize) {
   const int64_t v = 16 / (int64_t)esize;
   return aligned_to(p, 16) && D % v == 0 && (rows < 2 || rs % v == 0) && (groups < 2 || gs % v == 0);
+}
+
+static bool params_vectors_ok(const struct unirl_norm_desc* d) {
+  const size_t ps = (d->gain || d->bias) ? dtype_size(d->gain_dtype) : 4;
+  const int64_t v = 16 / (int64_t)ps;
+  return aligned_to(d->gain, 16) && aligned_to(d->bias, 16) && (!d->gain || d->gain_group_stride % v == 0) &&
+         (!d->bias || d->bias_group_stride % v == 0);
 }
 
 static int norm_check(const struct unirl_norm_desc* d) {
@@ -396,7 +527,7 @@ static NormArgs norm_args(const struct unirl_norm_desc* d, int64_t group0) {
   A.center = d->center;
   A.eps = (float)d->eps;
   A.inv_d = 1.0f / (float)d->D;
-  A.D = (int)d->D;
+  A.D = (uint32_t)d->D;
   A.rows = d->rows;
   A.mean = offset_f32(d->mean, group0 * d->rows);
   A.rstd = offset_f32(d->rstd, group0 * d->rows);
@@ -414,15 +545,15 @@ extern "C" int unirl_layer_norm_fwd(const struct unirl_norm_desc* d, void* y, vo
   if (!y) return UNIRL_E_NULL;
   const size_t es = dtype_size(d->dtype);
   if (!aligned_to(y, es)) return UNIRL_E_ALIGN;
-  const bool vectors = vectors_ok(d->x, d->x_group_stride, d->x_row_stride, d->D, d->groups, d->rows, es) && aligned_to(y, 16);
-  const NormShape S = norm_shape(d->D, d->dtype, vectors);
+  const bool vectors = vectors_ok(d->x, d->x_group_stride, d->x_row_stride, d->D, d->groups, d->rows, es) &&
+                       params_vectors_ok(d) && aligned_to(y, 16);
+  const NormShape S = norm_shape(d->D, d->dtype, vectors, false);
   for (int64_t g0 = 0; g0 < d->groups; g0 += kNormMaxGroups) {
     const int64_t ng = d->groups - g0 < kNormMaxGroups ? d->groups - g0 : kNormMaxGroups;
     NormArgs A = norm_args(d, g0);
     A.out = (char*)y + g0 * d->rows * d->D * (int64_t)es;
-    int64_t gx = S.one_wave ? (d->rows + kNormRowsPerBlock - 1) / kNormRowsPerBlock : d->rows;
-    if (gx > kNormMaxBlocks) gx = kNormMaxBlocks;
-    launch_norm(A, S, d->dtype, dim3((unsigned)gx, (unsigned)ng), false, false, (hipStream_t)stream);
+    const int64_t gx = norm_blocks(S, d->groups, d->rows, false);
+    launch_norm(A, S, d->dtype, dim3((unsigned)gx, (unsigned)ng), false, d->bias != nullptr, (hipStream_t)stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
@@ -431,7 +562,9 @@ extern "C" int unirl_layer_norm_fwd(const struct unirl_norm_desc* d, void* y, vo
 
 extern "C" size_t unirl_layer_norm_bwd_scratch_bytes(int64_t groups, int64_t rows, int64_t D) {
   if (groups <= 0 || rows <= 0 || D <= 0 || D > kNormMaxDim) return 0;
-  return (size_t)(groups * norm_bwd_blocks(groups, rows, D <= kWave * 32) * D) * 2 * sizeof(float);
+  // at least what norm_blocks gives for any layout of the operands
+  const int64_t want = (kNormMaxBlocks + groups - 1) / groups;
+  return (size_t)(groups * (want < rows ? want : rows) * D) * 2 * sizeof(float);
 }
 
 extern "C" int unirl_layer_norm_bwd(const struct unirl_norm_desc* d, const void* dy, int64_t dy_group_stride,
@@ -455,9 +588,9 @@ extern "C" int unirl_layer_norm_bwd(const struct unirl_norm_desc* d, const void*
     if (dy_group_stride < 0 || dy_row_stride < 0) return UNIRL_E_SHAPE;
     if (!aligned_to(dy, es) || !aligned_to(dx, es)) return UNIRL_E_ALIGN;
     const bool vectors = vectors_ok(d->x, d->x_group_stride, d->x_row_stride, d->D, d->groups, d->rows, es) &&
-                         vectors_ok(dy, dy_group_stride, dy_row_stride, d->D, d->groups, d->rows, es) && aligned_to(dx, 16);
-    const NormShape S = norm_shape(d->D, d->dtype, vectors);
-    blocks = norm_bwd_blocks(d->groups, d->rows, S.one_wave);
+                         vectors_ok(dy, dy_group_stride, dy_row_stride, d->D, d->groups, d->rows, es) && params_vectors_ok(d) && aligned_to(dx, 16);
+    const NormShape S = norm_shape(d->D, d->dtype, vectors, true);
+    blocks = norm_blocks(S, d->groups, d->rows, true);
     if (params) {
       if (!scratch || scratch_bytes < unirl_layer_norm_bwd_scratch_bytes(d->groups, d->rows, d->D)) return UNIRL_E_WORKSPACE;
       if (!aligned_to(scratch, 16)) return UNIRL_E_ALIGN;
@@ -483,19 +616,15 @@ extern "C" int unirl_layer_norm_bwd(const struct unirl_norm_desc* d, const void*
   const int64_t sets = per_group ? d->groups : 1;
   const int64_t n = empty ? 0 : (per_group ? blocks : d->groups * blocks);
   if (sets == 0) return UNIRL_OK;
-  const dim3 grid((unsigned)((d->D + 15) / 16), (unsigned)sets);
-  for (int which = 0; which < 2; ++which) {
-    void* out = which ? dbias : dgain;
-    if (!out) continue;
-    const float* p = part + (which ? part_bias : 0);
-    if (d->gain_dtype == UNIRL_F32)
-      hipLaunchKernelGGL((norm_param_kernel<float>), grid, dim3(256), 0, s, p, n, (int)d->D, (float*)out);
-    else if (d->gain_dtype == UNIRL_BF16)
-      hipLaunchKernelGGL((norm_param_kernel<bf16_t>), grid, dim3(256), 0, s, p, n, (int)d->D, (bf16_t*)out);
-    else
-      hipLaunchKernelGGL((norm_param_kernel<f16_t>), grid, dim3(256), 0, s, p, n, (int)d->D, (f16_t*)out);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-  }
-  return UNIRL_OK;
+  const dim3 grid((unsigned)((d->D + 31) / 32), (unsigned)sets, dbias ? 2 : 1);
+#define UNIRL_NORM_PARAM(O)                                                                                               \
+  hipLaunchKernelGGL((norm_param_kernel<O>), grid, dim3(1024), 0, s, part, part_bias, n, (uint32_t)d->D, (O*)dgain, (O*)dbias)
+  if (d->gain_dtype == UNIRL_F32)
+    UNIRL_NORM_PARAM(float);
+  else if (d->gain_dtype == UNIRL_BF16)
+    UNIRL_NORM_PARAM(bf16_t);
+  else
+    UNIRL_NORM_PARAM(f16_t);
+#undef UNIRL_NORM_PARAM
+  return (int)hipGetLastError();
 }
