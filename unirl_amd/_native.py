@@ -7,6 +7,8 @@ not been built, or a tensor does not live on a HIP device, the call raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
@@ -15,6 +17,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libunirl_hip.so"
+HOST_PATH = LIB_PATH.with_name("_unirl_torch_host.so")
 
 # enum unirl_dtype
 F32, BF16, F16 = 0, 1, 2
@@ -369,6 +372,29 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = argtypes
             _lib = handle
     return _lib
+
+
+_host = None
+
+
+def host():
+    """The C++ module that reads tensors for the operators over many tensors and the norms
+    (``csrc/torch_host.cpp``); loaded once, raises if it has not been built."""
+    global _host
+    if _host is not None:
+        return _host
+    lib()
+    with _lib_lock:
+        if _host is None:
+            if not HOST_PATH.exists():
+                raise RuntimeError(f"{HOST_PATH} is missing: build it with `python -m unirl_amd.build`")
+            loader = importlib.machinery.ExtensionFileLoader("_unirl_torch_host", str(HOST_PATH))
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+            loader.exec_module(module)
+            if module.abi_version != ABI_VERSION:
+                raise RuntimeError(f"{HOST_PATH} was built for ABI version {module.abi_version}: rebuild it")
+            _host = module
+    return _host
 
 
 class _Functions:

@@ -4,7 +4,8 @@
     python -m unirl_amd.build --tune     # measurement build beside it (libunirl_hip_tune.so)
 
 hipcc cross-compiles without a GPU.  Objects go to ``unirl_amd/lib/obj`` and the
-shared library to ``unirl_amd/lib/libunirl_hip.so``; both are git-ignored build
+shared library to ``unirl_amd/lib/libunirl_hip.so``; the C++ module that reads torch
+tensors for some of the Python operators goes beside it.  All are git-ignored build
 products.
 """
 
@@ -106,7 +107,31 @@ def build(verbose: bool = True, jobs: int | None = None, *, tune: bool = False, 
     os.replace(tmp, lib_path)
     if verbose:
         print(f"[unirl_amd.build] linked {lib_path}", flush=True)
+    if lib_path == LIB_PATH:
+        build_host(verbose=verbose)
     return lib_path
+
+
+def build_host(verbose: bool = True) -> Path:
+    """Compile ``csrc/torch_host.cpp`` (host code only) against the installed torch and the library."""
+    import sysconfig
+
+    from torch.utils import cpp_extension
+
+    out = LIB_DIR / "_unirl_torch_host.so"
+    if verbose:
+        print("[unirl_amd.build] g++ torch_host.cpp", flush=True)
+    rocm = Path(_hipcc()).resolve().parent.parent / "include"
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(rocm), "/opt/rocm/include"]
+    libs = Path(cpp_extension.__file__).resolve().parent.parent / "lib"
+    tmp = out.with_suffix(".so.tmp")
+    _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+          *[f"-I{d}" for d in includes], str(CSRC_DIR / "torch_host.cpp"), "-o", str(tmp), f"-L{LIB_DIR}", "-lunirl_hip", f"-L{libs}",
+          "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip", "-ltorch_hip", "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, out)
+    if verbose:
+        print(f"[unirl_amd.build] linked {out}", flush=True)
+    return out
 
 
 TUNE_LIB_PATH = LIB_DIR / "libunirl_hip_tune.so"

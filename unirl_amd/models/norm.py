@@ -7,7 +7,8 @@
   policy's output projection (the velocities that ``unirl/models/sd3/diffusion.py:467-497`` replays).
 
 The forward keeps the row's mean and reciprocal deviation (8 bytes a row) for the backward, which
-reads ``x`` and ``dy`` once and sums the gain's and bias's gradients in the same pass.
+reads ``x`` and ``dy`` once and sums the gain's and bias's gradients in the same pass.  Forward and
+backward are one C++ autograd node (``csrc/torch_host.cpp``); the backward is not differentiable.
 """
 
 from __future__ import annotations
@@ -15,35 +16,8 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from .. import ops
-
-
-class _NormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps: float, rms: bool, unit_offset: bool):
-        y, mean, rstd = ops.layer_norm(x, weight, bias, eps=eps, rms=rms, unit_offset=unit_offset, want_stats=True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.form = (rms, unit_offset)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        rms, unit_offset = ctx.form
-        dx, dw, db = ops.layer_norm_bwd(
-            dy, x, mean, rstd, weight, bias, rms=rms, unit_offset=unit_offset,
-            want_dx=ctx.needs_input_grad[0], want_dweight=ctx.needs_input_grad[1], want_dbias=ctx.needs_input_grad[2],
-        )
-        return dx, dw, db, None, None, None
-
-
-def _norm(x, weight, bias, eps, rms, unit_offset) -> torch.Tensor:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _NormFn.apply(x, weight, bias, float(eps), rms, unit_offset)
-    return ops.layer_norm(x, weight, bias, eps=eps, rms=rms, unit_offset=unit_offset)[0]
+from .. import _native as N
 
 
 def layer_norm(
@@ -54,7 +28,7 @@ def layer_norm(
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None and p.dim() != 1:
             raise ValueError(f"{name} must be [D]; got {tuple(p.shape)} (modulated_layer_norm takes one row per sample)")
-    return _norm(x, weight, bias, eps, False, False)
+    return N.host().norm(x, weight, bias, eps, False, False)
 
 
 def rms_norm(
@@ -65,7 +39,7 @@ def rms_norm(
     not preceded by a rounding to 16 bits); differentiable in ``x`` and ``weight``."""
     if weight is not None and weight.dim() != 1:
         raise ValueError(f"weight must be [D]; got {tuple(weight.shape)}")
-    return _norm(x, weight, None, eps, True, unit_offset)
+    return N.host().norm(x, weight, None, eps, True, unit_offset)
 
 
 def modulated_layer_norm(x: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
@@ -80,7 +54,7 @@ def modulated_layer_norm(x: torch.Tensor, scale: torch.Tensor, shift: torch.Tens
         if p.dim() < 2 or (p.shape[0], p.shape[-1]) != rows or p.numel() != rows[0] * rows[1]:
             raise ValueError(f"{name} must be [{rows[0]}, {rows[1]}]; got {tuple(p.shape)}")
         given[name] = p if p.dim() == 2 else p.reshape(rows)
-    return _norm(x, given["scale"], given["shift"], eps, False, True)
+    return N.host().norm(x, given["scale"], given["shift"], eps, False, True)
 
 
 __all__ = ["layer_norm", "modulated_layer_norm", "rms_norm"]

@@ -7,7 +7,6 @@ API (``unirl_amd.sde``, ``unirl_amd.algorithms``, ...) is built on these.
 
 from __future__ import annotations
 
-import array
 import ctypes
 import functools
 import math
@@ -1504,71 +1503,6 @@ def expand_groups(unique: torch.Tensor, group_of: torch.Tensor, dtype: torch.dty
 NORM_MAX_DIM = 32768  # elements of a row
 
 
-def _norm_rows(x: torch.Tensor, per_group: bool) -> Tuple[torch.Tensor, int, int, int, int]:
-    """``(tensor, groups, rows, group stride, row stride)`` of ``x [..., D]``: read in place when its
-    leading dimensions are at most two runs of equally spaced rows (with ``per_group`` dimension 0 is
-    the groups), else from a contiguous copy.  Shared gains leave one partial sum per group, so many
-    short groups are copied together as well."""
-    D = x.shape[-1]
-    n = x.numel() // D if D else 0
-    if not x.is_contiguous():
-        runs: List[List[int]] = []  # [size, stride], outermost first; dimension 0 stays apart for groups
-        for i, (size, stride) in enumerate(zip(x.shape[:-1], x.stride()[:-1])):
-            if size == 1 and not (per_group and i == 0):
-                continue
-            if runs and not (per_group and len(runs) == 1) and runs[-1][1] == stride * size:
-                runs[-1] = [runs[-1][0] * size, stride]
-            else:
-                runs.append([size, stride])
-        if (x.stride(-1) == 1 or D == 1) and len(runs) <= 2 and (per_group or len(runs) < 2 or runs[0][0] <= 256):
-            while len(runs) < 2:
-                runs.insert(len(runs) if per_group else 0, [1, 0])
-            (G, gs), (R, rs) = runs
-            return x, G, R, gs, rs
-        x = x.contiguous()
-    if per_group:
-        G = x.shape[0]
-        R = n // G if G else 0
-        return x, G, R, R * D, D
-    return x, 1, n, 0, D
-
-
-def _norm_param(p: Optional[torch.Tensor], x: torch.Tensor, name: str) -> Tuple[Optional[torch.Tensor], bool]:
-    """A gain or bias with its elements adjacent, and whether it has one row per group."""
-    if p is None:
-        return None, False
-    N.require_device(p, name)
-    if p.device != x.device:
-        raise ValueError(f"{name} lives on {p.device}, x on {x.device}")
-    D = x.shape[-1]
-    if tuple(p.shape) != (D,) and not (p.dim() == 2 and x.dim() >= 2 and tuple(p.shape) == (x.shape[0], D)):
-        raise ValueError(f"{name} must be [{D}] or [{x.shape[0] if x.dim() > 1 else 'groups'}, {D}]; got {tuple(p.shape)}")
-    N.dtype_code(p.dtype)
-    return (p if p.stride(-1) == 1 or D <= 1 else p.contiguous()), p.dim() == 2
-
-
-def _norm_desc(x, weight, bias, eps, rms, unit_offset):
-    """``(desc, tensor read, per_group)`` with everything but the statistics filled in."""
-    N.require_device(x, "x")
-    code = N.dtype_code(x.dtype)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must be [..., D] with D >= 1; got {tuple(x.shape)}")
-    w, w_rows = _norm_param(weight, x, "weight")
-    b, b_rows = _norm_param(bias, x, "bias")
-    if w is not None and b is not None and (w.dtype != b.dtype or w_rows != b_rows):
-        raise ValueError(f"weight and bias differ: {w.dtype} {tuple(w.shape)}, {b.dtype} {tuple(b.shape)}")
-    per_group = w_rows or b_rows
-    t, G, R, gs, rs = _norm_rows(x, per_group)
-    p = w if w is not None else b
-    desc = N.NormDesc(
-        x=N.ptr(t), dtype=code, x_group_stride=gs, x_row_stride=rs, groups=G, rows=R, D=x.shape[-1], gain=N.ptr(w), bias=N.ptr(b),
-        gain_dtype=N.F32 if p is None else N.dtype_code(p.dtype),
-        gain_group_stride=w.stride(0) if w_rows else 0, bias_group_stride=b.stride(0) if b_rows else 0,
-        gain_offset=1.0 if unit_offset else 0.0, center=0 if rms else 1, eps=float(eps),
-    )
-    return desc, (t, w, b), per_group
-
-
 def layer_norm(
     x: torch.Tensor,
     weight: Optional[torch.Tensor] = None,
@@ -1587,17 +1521,8 @@ def layer_norm(
     in one dtype of their own.  ``mean`` (``None`` for ``rms``) and ``rstd`` are fp32 ``x.shape[:-1]``,
     only with ``want_stats``.  ``x`` may be a view whose rows are equally spaced (``hidden[:, a:b]``).
     """
-    desc, held, _ = _norm_desc(x, weight, bias, eps, rms, unit_offset)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if want_stats:
-        rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        mean = None if rms else torch.empty_like(rstd)
-        desc.mean, desc.rstd = N.ptr(mean), N.ptr(rstd)
-    if y.numel():
-        with N.on_device(x.device):
-            rc = N.F.unirl_layer_norm_fwd(ctypes.byref(desc), N.ptr(y), N.current_stream(x.device))
-        N.check(rc, "unirl_layer_norm_fwd")
+    rc, y, mean, rstd = N.host().layer_norm(x, weight, bias, eps, rms, unit_offset, want_stats)
+    N.check(rc, "unirl_layer_norm_fwd")
     return y, mean, rstd
 
 
@@ -1619,35 +1544,9 @@ def layer_norm_bwd(
     of ``want_stats``.  ``dx`` has ``x``'s dtype; the parameters' gradients have their shapes and dtype,
     summed in fp32 over the rows that read them, in an order that depends on the shape alone.  ``bias``
     gives its shape and dtype only; a gradient whose parameter is ``None`` is ``None``."""
-    desc, held, per_group = _norm_desc(x, weight, bias, 0.0, rms, unit_offset)
-    if dy.shape != x.shape:
-        raise ValueError(f"dy {tuple(dy.shape)} != x {tuple(x.shape)}")
-    if rstd.shape != x.shape[:-1] or (not rms and (mean is None or mean.shape != x.shape[:-1])):
-        raise ValueError("mean and rstd must be the statistics of this x")
-    device = x.device
-    rstd = N.as_operand(rstd, torch.float32, device)
-    mean = None if rms else N.as_operand(mean, torch.float32, device)
-    desc.mean, desc.rstd = N.ptr(mean), N.ptr(rstd)
-    g = dy if dy.dtype == x.dtype and dy.device == device else dy.detach().to(device=device, dtype=x.dtype)
-    g, G, R, gs, rs = _norm_rows(g, per_group)
-    if (G, R) != (desc.groups, desc.rows):  # the two are cut into groups unlike each other
-        g = g.contiguous()
-        R, G = desc.rows, desc.groups
-        gs, rs = R * desc.D, desc.D
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_dx else None
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=device) if want_dweight and weight is not None else None
-    db = torch.empty(bias.shape, dtype=bias.dtype, device=device) if want_dbias and bias is not None else None
-    if dx is None and dw is None and db is None:
-        return None, None, None
-    scratch = nbytes = None
-    if dw is not None or db is not None:
-        nbytes = int(N.F.unirl_layer_norm_bwd_scratch_bytes(desc.groups, desc.rows, desc.D))
-        scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
-    with N.on_device(device):
-        rc = N.F.unirl_layer_norm_bwd(
-            ctypes.byref(desc), N.ptr(g), gs, rs, N.ptr(dx) if dx is not None and dx.numel() else None, N.ptr(dw), N.ptr(db),
-            int(per_group), N.ptr(scratch), nbytes or 0, N.current_stream(device),
-        )
+    rc, dx, dw, db = N.host().layer_norm_bwd(
+        dy, x, mean, rstd, weight, bias, rms, unit_offset, want_dx, want_dweight, want_dbias
+    )
     N.check(rc, "unirl_layer_norm_bwd")
     return dx, dw, db
 
@@ -1665,25 +1564,7 @@ def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     the sizes alone; Inf and NaN propagate.  Two launches for up to 160 tensors, one more for every
     further 160; nothing is copied from the host and nothing synchronises.
     """
-    ts = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    if not ts:
-        raise ValueError("grad_norm needs at least one tensor")
-    device = ts[0].device
-    N.require_device(ts[0], "grads[0]")
-    if any(t.device != device for t in ts):
-        raise ValueError("grad_norm: the tensors live on different devices")
-    n = len(ts)
-    ptrs = array.array("Q", [t.data_ptr() for t in ts])
-    numels = array.array("q", [t.numel() for t in ts])
-    codes = array.array("i", [N.dtype_code(t.dtype) for t in ts])
-    out = torch.empty((), dtype=torch.float32, device=device)
-    # scratch of this call alone: calls on other streams, and graphs, never share it
-    ws = torch.empty(int(N.F.unirl_workspace_bytes()), dtype=torch.uint8, device=device)
-    with N.on_device(device):
-        rc = N.F.unirl_grad_norm(
-            ptrs.buffer_info()[0], numels.buffer_info()[0], codes.buffer_info()[0], n, N.ptr(out), N.ptr(ws), ws.numel(),
-            N.current_stream(device),
-        )
+    rc, out = N.host().grad_norm(grads)
     N.check(rc, "unirl_grad_norm")
     return out
 
@@ -1761,26 +1642,18 @@ def adamw_step(
     have them move, pass ``control`` from :func:`adamw_advance` instead of ``lr``, ``step``, ``weight_decay``,
     ``seed``, ``grad_norm``, ``max_norm`` and ``skip_nonfinite``.
     """
-    n = len(params)
-    states8 = exp_avg_scales is not None or exp_avg_sq_scales is not None
-    lists = {"grads": grads, "exp_avgs": exp_avgs, "exp_avg_sqs": exp_avg_sqs}
-    if masters is not None:
-        lists["masters"] = masters
-    if states8:
-        if exp_avg_scales is None or exp_avg_sq_scales is None:
-            raise ValueError("8-bit moments need exp_avg_scales and exp_avg_sq_scales")
-        lists.update(exp_avg_scales=exp_avg_scales, exp_avg_sq_scales=exp_avg_sq_scales)
-    if index_bases is not None:
-        lists["index_bases"] = index_bases
-    for name, items in lists.items():
-        if len(items) != n:
-            raise ValueError(f"{name} has {len(items)} entries for {n} params")
     b1, b2 = _adamw_hyper(betas, eps, weight_decay)
+    if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
+        raise ValueError("8-bit moments need exp_avg_scales and exp_avg_sq_scales")
+    n = len(params)
+    for name, items in (("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs), ("masters", masters),
+                        ("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales), ("index_bases", index_bases)):
+        if items is not None and len(items) != n:
+            raise ValueError(f"{name} has {len(items)} entries for {n} params")
     if n == 0:
         return
-    device, dtype = params[0].device, params[0].dtype
+    device = params[0].device
     N.require_device(params[0], "params[0]")
-    code = N.dtype_code(dtype)
     if control is not None:
         if step is not None or lr is not None or grad_norm is not None or max_norm is not None or skip_nonfinite:
             raise ValueError("control already holds lr, step and the clip factor: pass either those or control")
@@ -1788,52 +1661,12 @@ def adamw_step(
     elif lr is None or step is None or int(step) < 1:
         raise ValueError(f"adamw_step needs lr and a step of at least 1 (or control); got lr={lr}, step={step}")
     bound = _clip_args(grad_norm, max_norm, skip_nonfinite, device)
-    numels = [p.numel() for p in params]
-    _same_numel("params", params, numels, dtype, device)
-    gs = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    gdtype = gs[0].dtype
-    if gdtype != dtype and gdtype != torch.float32:
-        raise TypeError(f"gradients of {dtype} parameters must be {dtype} or float32; got {gdtype}")
-    _same_numel("grads", gs, numels, gdtype, device)
-    sdtype = torch.uint8 if states8 else torch.float32
-    _same_numel("exp_avgs", exp_avgs, numels, sdtype, device)
-    _same_numel("exp_avg_sqs", exp_avg_sqs, numels, sdtype, device)
-    if masters is not None:
-        if dtype == torch.float32:
-            raise ValueError("masters are for 16-bit params: fp32 params hold their own values")
-        _same_numel("masters", masters, numels, torch.float32, device)
-    zeros = [0] * n
-    scales = [zeros, zeros]
-    if states8:
-        blocks = [-(-k // ADAMW_BLOCK) for k in numels]
-        for name, items in (("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales)):
-            _same_numel(name, items, blocks, torch.uint8, device)
-        scales = [[t.data_ptr() for t in exp_avg_scales], [t.data_ptr() for t in exp_avg_sq_scales]]
-        if index_bases is None:
-            index_bases, at = [], 0
-            for k in blocks:
-                index_bases.append(at)
-                at += k * ADAMW_BLOCK
-    addresses = [p.data_ptr() for p in params]
-    if len(set(a for a, k in zip(addresses, numels) if k)) != n - numels.count(0):
-        raise ValueError("the same parameter appears more than once")
-    columns = (
-        addresses, [g.data_ptr() for g in gs], [t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs],
-        zeros if masters is None else [t.data_ptr() for t in masters], *scales, numels,
-        zeros if index_bases is None else index_bases,
+    rc = N.host().adamw_step(
+        params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_scales, exp_avg_sq_scales, index_bases,
+        0.0 if lr is None else lr, b1, b2, eps, weight_decay, 0 if step is None else int(step), int(seed) & 0xFFFFFFFF, grad_norm,
+        bound, int(bool(skip_nonfinite)), control,
     )
-    table = array.array("q", [v for row in zip(*columns) for v in row])  # struct unirl_adamw_tensor[n]
-    q = N.AdamwParams(
-        param_dtype=code, grad_dtype=N.dtype_code(gdtype), state_bits=8 if states8 else 32, use_master=int(masters is not None),
-        lr=0.0 if lr is None else float(lr), beta1=b1, beta2=b2, eps=float(eps), weight_decay=float(weight_decay),
-        step=0 if step is None else int(step), seed=int(seed) & 0xFFFFFFFF, grad_norm=N.ptr(grad_norm), max_norm=bound,
-        skip_nonfinite=int(bool(skip_nonfinite)), control=N.ptr(control),
-    )
-    with N.on_device(device):
-        rc = N.F.unirl_adamw_step(table.buffer_info()[0], n, ctypes.byref(q), N.current_stream(device))
     N.check(rc, "unirl_adamw_step")
-    # written behind autograd's back: whoever saved a parameter for a backward has to notice
-    torch.autograd.graph.increment_version(params)
 
 
 def adamw_advance(
