@@ -1,7 +1,7 @@
 // The optimizer's side of a policy update over many tensors at once: the global norm of the
 // gradients and the AdamW step with its moments in 32 bits or in 8.
 //
-// Tables of tensors ride in the kernel arguments (48 or 160 tensors a launch, under 4 KB), so a call
+// Tables of tensors ride in the kernel arguments (50 to 160 tensors a launch, under 4 KB), so a call
 // copies nothing to the device, keeps nothing between calls and can be captured into a graph.
 // Workgroup b finds its tensor by comparing b with the tensors' first workgroups, one per lane, and
 // counting the lanes that are not beyond it: one load and a ballot instead of a search.
@@ -111,12 +111,14 @@ __global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* pa
 // ---------------------------------------------------------------------------
 // AdamW
 // ---------------------------------------------------------------------------
-constexpr int kAdamTensors = 48;
 constexpr int kAdamThreads = 256;
 constexpr int kQuantBlock = 256;  // elements that share a scale: one wavefront's four elements a lane
-constexpr int kAdamUnroll = 4;    // blocks of one wavefront
+// Blocks of one wavefront, whose loads are in flight together.  With 32-bit moments one block is
+// enough (eight wavefronts a SIMD keep the memory busy) and the shorter code is fetched sooner: a launch over 1.6 M elements takes 10.2 us with one block, 10.4 with two, 11.3 with four,
+// one over 400 M 2.02, 2.10, 2.06 ms.  With 8-bit moments: 9.3 / 9.6 / 11.3 us and 1.20 / 1.14 / 1.16 ms.
+constexpr int adam_unroll(int bits) { return bits == 32 ? 1 : 2; }
 constexpr int64_t kMaxGrid = 0xffffff;  // workgroups of 256 threads: a launch counts its threads in 32 bits
-constexpr int kAdamChunk = kAdamThreads / kWave * kAdamUnroll * kQuantBlock;
+constexpr int adam_chunk(int bits) { return kAdamThreads / kWave * adam_unroll(bits) * kQuantBlock; }
 
 // The scalars of one step, as the kernels read them (the first fields of the caller's control buffer).
 struct AdamControl {
@@ -129,17 +131,41 @@ struct AdamControl {
 };
 static_assert(sizeof(AdamControl) <= UNIRL_ADAMW_CONTROL_BYTES, "control buffer");
 
-struct AdamArgs {
-  struct unirl_adamw_tensor t[kAdamTensors];
-  uint32_t first[kAdamTensors];
-  uint64_t aligned;  // bit per tensor: every pointer suits the vector accesses
+// A tensor's entry holds what its kind of step reads, so that as many as possible share a launch: 90
+// (32-bit moments) to 52 (8-bit moments and a master).
+struct AdamMaster {
+  float* master;
+};
+struct AdamBytes {
+  uint8_t *exp_avg_scale, *exp_avg_sq_scale;
+  int64_t index_base;
+};
+template <int>
+struct Nothing {};
+template <int BITS, bool MASTER>
+struct AdamEntry : std::conditional<MASTER, AdamMaster, Nothing<0>>::type, std::conditional<BITS == 8, AdamBytes, Nothing<1>>::type {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  int64_t numel2;  // twice the number of elements; odd: every pointer suits the vector accesses
+};
+struct AdamCommon {
   const AdamControl* control;
   const float* norm;
   AdamControl host;
   float max_norm, beta1, beta2, one_minus_beta1, one_minus_beta2, eps;
   int skip_nonfinite;
 };
-static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
+template <int BITS, bool MASTER>
+struct AdamArgs : AdamCommon {
+  static constexpr int kTensors = (4096 - 96) / (int)(sizeof(AdamEntry<BITS, MASTER>) + 4) / 2 * 2;
+  uint32_t first[kTensors];  // first workgroup of each tensor; above the grid's size behind the last
+  AdamEntry<BITS, MASTER> t[kTensors];
+};
+static_assert(sizeof(AdamArgs<32, false>) <= 4096 && sizeof(AdamArgs<32, true>) <= 4096 && sizeof(AdamArgs<8, false>) <= 4096 &&
+                  sizeof(AdamArgs<8, true>) <= 4096,
+              "kernel arguments");
 
 // A bijection of 32-bit words whose output bits each depend on all input bits: xor-shifts and odd
 // products, with the fractions of sqrt(2) and sqrt(3) as constants (flipping any input bit flips each
@@ -203,7 +229,7 @@ template <typename P, typename G, int BITS, bool MASTER>
 struct AdamLane {
   float p[4], g[4], m[4], v[4];
 
-  __device__ __forceinline__ void update(const AdamArgs& A, const AdamControl& C) {
+  __device__ __forceinline__ void update(const AdamCommon& A, const AdamControl& C) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float gc = g[k] * C.clip;
@@ -260,12 +286,146 @@ __device__ __forceinline__ void decode_v4(uint32_t codes, float scale, float (&o
   for (int k = 0; k < 4; ++k) o[k] = f16_bits_to_f32(((codes >> (8 * k)) & 0xffu) << 7) * scale;
 }
 
+// Where one wavefront's elements lie and how its lanes reach them: four adjacent elements in one access,
+// or element by element through buffer descriptors that end with the tensor (loads behind the end give
+// zeros, stores there are dropped), so that neither stands behind a condition.
+template <typename T, bool VECTORS>
+struct Span {
+  T* p;
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ Span(const void* base, int64_t e0, uint32_t count) : p((T*)base + e0) {
+    if constexpr (!VECTORS) r = __builtin_amdgcn_make_buffer_rsrc(p, 0, count * (uint32_t)sizeof(T), 0x00020000);
+  }
+  __device__ __forceinline__ void load(uint32_t i, float (&o)[4]) const {
+    if constexpr (VECTORS) {
+      Vec<T, 4>::load(p + i, o);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) {
+          o[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, (i + k) * 4, 0, 0));
+        } else {
+          T t;
+          t.bits = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, (i + k) * 2, 0, 0);
+          o[k] = Elem<T>::load(&t);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint32_t i, const float (&o)[4]) const {
+    if constexpr (VECTORS) {
+      Vec<T, 4>::store(p + i, o);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) {
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[k]), r, (i + k) * 4, 0, 0);
+        } else {
+          T t;
+          Elem<T>::store(&t, o[k]);
+          __builtin_amdgcn_raw_buffer_store_b16((short)t.bits, r, (i + k) * 2, 0, 0);
+        }
+      }
+    }
+  }
+};
+template <bool VECTORS>
+struct Span<uint8_t, VECTORS> {
+  uint8_t* p;
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ Span(const void* base, int64_t e0, uint32_t count) : p((uint8_t*)base + e0) {
+    if constexpr (!VECTORS) r = __builtin_amdgcn_make_buffer_rsrc(p, 0, count, 0x00020000);
+  }
+  __device__ __forceinline__ uint32_t load(uint32_t i) const {
+    if constexpr (VECTORS) return __builtin_nontemporal_load((const uint32_t*)(p + i));
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w |= (uint32_t)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, i + k, 0, 0) << (8 * k);
+    return w;
+  }
+  __device__ __forceinline__ void store(uint32_t i, uint32_t w) const {
+    if constexpr (VECTORS) {
+      __builtin_nontemporal_store(w, (uint32_t*)(p + i));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) __builtin_amdgcn_raw_buffer_store_b8((char)(w >> (8 * k)), r, i + k, 0, 0);
+    }
+  }
+};
+
+// One wavefront's blocks of 256 elements from e0 on: all their loads are in flight before the first
+// is used.  `count` of the elements exist (VECTORS: all).
+template <typename P, typename G, int BITS, bool MASTER, bool VECTORS>
+__device__ __forceinline__ void adamw_blocks(const AdamCommon& A, const AdamControl& C, const AdamEntry<BITS, MASTER>& T, int64_t e0,
+                                             uint32_t count, uint32_t lane) {
+  constexpr int kUnroll = adam_unroll(BITS);
+  const Span<P, VECTORS> param(T.param, e0, count);
+  const Span<G, VECTORS> grad(T.grad, e0, count);
+  const void* master_base = T.param;
+  if constexpr (MASTER) master_base = T.master;
+  const Span<float, VECTORS> master(master_base, e0, count);
+  using S = typename std::conditional<BITS == 32, float, uint8_t>::type;
+  const Span<S, VECTORS> avg(T.exp_avg, e0, count), sq(T.exp_avg_sq, e0, count);
+  const int64_t block0 = e0 / kQuantBlock;
+  AdamLane<P, G, BITS, MASTER> L[kUnroll];
+  uint32_t cm[kUnroll], cv[kUnroll], sm[kUnroll], sv[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t i = u * kQuantBlock + lane * 4;
+    grad.load(i, L[u].g);
+    if constexpr (MASTER)
+      master.load(i, L[u].p);
+    else
+      param.load(i, L[u].p);
+    if constexpr (BITS == 32) {
+      avg.load(i, L[u].m);
+      sq.load(i, L[u].v);
+    } else {
+      cm[u] = avg.load(i);
+      cv[u] = sq.load(i);
+      const int64_t block = block0 + (VECTORS || u * kQuantBlock < count ? u : 0);  // one that exists
+      sm[u] = T.exp_avg_scale[block];
+      sv[u] = T.exp_avg_sq_scale[block];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    if (!VECTORS && u * kQuantBlock >= count) break;
+    const uint32_t i = u * kQuantBlock + lane * 4;
+    if constexpr (BITS == 8) {
+      decode_m4(cm[u], scale_of(sm[u]), L[u].m);
+      decode_v4(cv[u], scale_of(sv[u]), L[u].v);
+    }
+    L[u].update(A, C);
+    if constexpr (MASTER) master.store(i, L[u].p);
+    param.store(i, L[u].p);
+    if constexpr (BITS == 32) {
+      avg.store(i, L[u].m);
+      sq.store(i, L[u].v);
+    } else {
+      // what lies behind the tensor's end stays out of the block's maximum, whatever the clip factor is
+      if constexpr (!VECTORS)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k >= count) L[u].m[k] = L[u].v[k] = 0.0f;
+      const uint64_t index = (uint64_t)T.index_base + (uint64_t)e0 + i;
+      uint32_t wm, wv, km, kv;
+      L[u].encode((uint32_t)index, C.key + (uint32_t)(index >> 32) * 0x9E3779B9u, wm, wv, km, kv);
+      avg.store(i, wm);
+      sq.store(i, wv);
+      if (lane == 0) {
+        T.exp_avg_scale[block0 + u] = (uint8_t)km;
+        T.exp_avg_sq_scale[block0 + u] = (uint8_t)kv;
+      }
+    }
+  }
+}
+
 // Bound by HBM: 28 bytes an element with 32-bit moments and a master, 10 with 8-bit moments and a
-// 16-bit parameter.  One wavefront takes four blocks of 256 elements, four elements a lane, so that
-// all loads of 1024 elements are in flight before the first is used; a block's maximum is then one
-// reduction inside a wavefront.
+// 16-bit parameter.  A lane takes four elements of a block, so that a block's maximum is one reduction
+// inside a wavefront.
 template <typename P, typename G, int BITS, bool MASTER>
-__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs A) {
+__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs<BITS, MASTER> A) {
   AdamControl C = A.host;
   if (A.control) {
     C = *A.control;
@@ -275,125 +435,18 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs A) {
     C.skip = A.skip_nonfinite && !finite_f32(norm);
   }
   if (C.skip) return;
-  const int t = find_tensor<kAdamTensors>(A.first, blockIdx.x);
-  const struct unirl_adamw_tensor& T = A.t[t];
-  const int64_t n = T.numel;
+  constexpr int kElements = adam_unroll(BITS) * kQuantBlock;  // of one wavefront
+  const int t = find_tensor<AdamArgs<BITS, MASTER>::kTensors>(A.first, blockIdx.x);
+  const AdamEntry<BITS, MASTER>& T = A.t[t];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t e0 = (int64_t)(blockIdx.x - A.first[t]) * kAdamChunk + (int64_t)wave * (kAdamUnroll * kQuantBlock);
-  if (e0 >= n) return;
-  P* param = (P*)T.param;
-  const G* grad = (const G*)T.grad;
-  float* master = (float*)T.master;
-  using Lane = AdamLane<P, G, BITS, MASTER>;
-
-  if (((A.aligned >> t) & 1) && e0 + kAdamUnroll * kQuantBlock <= n) {
-    Lane L[kAdamUnroll];
-    uint32_t cm[kAdamUnroll], cv[kAdamUnroll], sm[kAdamUnroll], sv[kAdamUnroll];
-#pragma unroll
-    for (int u = 0; u < kAdamUnroll; ++u) {
-      const int64_t i = e0 + u * kQuantBlock + lane * 4;
-      Vec<G, 4>::load(grad + i, L[u].g);
-      if constexpr (MASTER)
-        Vec<float, 4>::load(master + i, L[u].p);
-      else
-        Vec<P, 4>::load(param + i, L[u].p);
-      if constexpr (BITS == 32) {
-        Vec<float, 4>::load((const float*)T.exp_avg + i, L[u].m);
-        Vec<float, 4>::load((const float*)T.exp_avg_sq + i, L[u].v);
-      } else {
-        cm[u] = __builtin_nontemporal_load((const uint32_t*)((const uint8_t*)T.exp_avg + i));
-        cv[u] = __builtin_nontemporal_load((const uint32_t*)((const uint8_t*)T.exp_avg_sq + i));
-        sm[u] = T.exp_avg_scale[e0 / kQuantBlock + u];
-        sv[u] = T.exp_avg_sq_scale[e0 / kQuantBlock + u];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kAdamUnroll; ++u) {
-      const int64_t i = e0 + u * kQuantBlock + lane * 4;
-      if constexpr (BITS == 8) {
-        decode_m4(cm[u], scale_of(sm[u]), L[u].m);
-        decode_v4(cv[u], scale_of(sv[u]), L[u].v);
-      }
-      L[u].update(A, C);
-      if constexpr (MASTER) Vec<float, 4>::store(master + i, L[u].p);
-      Vec<P, 4>::store(param + i, L[u].p);
-      if constexpr (BITS == 32) {
-        Vec<float, 4>::store((float*)T.exp_avg + i, L[u].m);
-        Vec<float, 4>::store((float*)T.exp_avg_sq + i, L[u].v);
-      } else {
-        const uint64_t index = (uint64_t)T.index_base + (uint64_t)i;
-        uint32_t wm, wv, km, kv;
-        L[u].encode((uint32_t)index, C.key + (uint32_t)(index >> 32) * 0x9E3779B9u, wm, wv, km, kv);
-        __builtin_nontemporal_store(wm, (uint32_t*)((uint8_t*)T.exp_avg + i));
-        __builtin_nontemporal_store(wv, (uint32_t*)((uint8_t*)T.exp_avg_sq + i));
-        if (lane == 0) {
-          T.exp_avg_scale[e0 / kQuantBlock + u] = (uint8_t)km;
-          T.exp_avg_sq_scale[e0 / kQuantBlock + u] = (uint8_t)kv;
-        }
-      }
-    }
-    return;
-  }
-
-  // element by element: a tensor's last blocks, and tensors whose pointers do not suit the vectors
-  for (int u = 0; u < kAdamUnroll; ++u) {
-    const int64_t b = e0 + u * kQuantBlock;
-    if (b >= n) break;
-    const int64_t i = b + lane * 4;
-    Lane L;
-    float sm = 0.0f, sv = 0.0f;
-    if constexpr (BITS == 8) {
-      sm = scale_of(T.exp_avg_scale[b / kQuantBlock]);
-      sv = scale_of(T.exp_avg_sq_scale[b / kQuantBlock]);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bool in = i + k < n;
-      L.g[k] = in ? Elem<G>::load(grad + i + k) : 0.0f;
-      if constexpr (MASTER)
-        L.p[k] = in ? master[i + k] : 0.0f;
-      else
-        L.p[k] = in ? Elem<P>::load(param + i + k) : 0.0f;
-      if constexpr (BITS == 32) {
-        L.m[k] = in ? ((const float*)T.exp_avg)[i + k] : 0.0f;
-        L.v[k] = in ? ((const float*)T.exp_avg_sq)[i + k] : 0.0f;
-      } else {
-        float om[4], ov[4];
-        decode_m4(in ? ((const uint8_t*)T.exp_avg)[i + k] : 0u, sm, om);
-        decode_v4(in ? ((const uint8_t*)T.exp_avg_sq)[i + k] : 0u, sv, ov);
-        L.m[k] = om[0];
-        L.v[k] = ov[0];
-      }
-    }
-    L.update(A, C);
-    uint32_t wm = 0, wv = 0, km = 0, kv = 0;
-    if constexpr (BITS == 8) {
-      // what lies behind the tensor's end stays out of the block's maximum, whatever the clip factor is
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (i + k >= n) L.m[k] = L.v[k] = 0.0f;
-      const uint64_t index = (uint64_t)T.index_base + (uint64_t)i;
-      L.encode((uint32_t)index, C.key + (uint32_t)(index >> 32) * 0x9E3779B9u, wm, wv, km, kv);
-      if (lane == 0) {
-        T.exp_avg_scale[b / kQuantBlock] = (uint8_t)km;
-        T.exp_avg_sq_scale[b / kQuantBlock] = (uint8_t)kv;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (i + k >= n) continue;
-      if constexpr (MASTER) master[i + k] = L.p[k];
-      Elem<P>::store(param + i + k, L.p[k]);
-      if constexpr (BITS == 32) {
-        ((float*)T.exp_avg)[i + k] = L.m[k];
-        ((float*)T.exp_avg_sq)[i + k] = L.v[k];
-      } else {
-        ((uint8_t*)T.exp_avg)[i + k] = (uint8_t)(wm >> (8 * k));
-        ((uint8_t*)T.exp_avg_sq)[i + k] = (uint8_t)(wv >> (8 * k));
-      }
-    }
-  }
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  const int64_t e0 = (int64_t)(blockIdx.x - A.first[t]) * adam_chunk(BITS) + (int64_t)wave * kElements;
+  const int64_t left = (T.numel2 >> 1) - e0;
+  if (left <= 0) return;
+  if ((T.numel2 & 1) && left >= kElements)
+    adamw_blocks<P, G, BITS, MASTER, true>(A, C, T, e0, kElements, lane);
+  else
+    adamw_blocks<P, G, BITS, MASTER, false>(A, C, T, e0, left < kElements ? (uint32_t)left : kElements, lane);
 }
 
 struct AdamScalars {
@@ -430,54 +483,113 @@ __global__ void adamw_advance_kernel(int64_t* step, AdamControl* control, AdamSc
   if (!skip) *step = t;
 }
 
-// The values that 8-bit moments stand for: four elements a lane, one block a wavefront.
+// The values that 8-bit moments stand for: eight elements a lane (a lane's stores are 16 bytes in 16-bit
+// types), four times; blockIdx.y: m, v.
+constexpr int kMomentsChunk = 256 * 8 * 4;
 template <typename O>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t* m, const uint8_t* v, const uint8_t* sm,
                                                             const uint8_t* sv, int64_t n, O* out_m, O* out_v, int aligned) {
-  for (int64_t block = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave; block * kQuantBlock < n; block += (int64_t)gridDim.x * 4)
+  const bool second = blockIdx.y != 0;
+  const uint8_t *codes = second ? v : m, *scales = second ? sv : sm;
+  O* out = second ? out_v : out_m;
+  if (!out) return;
+  const auto decode = [second](uint32_t w, float scale, float (&o)[4]) {
+    if (second)
+      decode_v4(w, scale, o);
+    else
+      decode_m4(w, scale, o);
+  };
+  for (int64_t e0 = (int64_t)blockIdx.x * kMomentsChunk; e0 < n; e0 += (int64_t)gridDim.x * kMomentsChunk) {
+    if (aligned && e0 + kMomentsChunk <= n) {
+      u32x2 w[4];
+      uint32_t s[4];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const int64_t i = block * kQuantBlock + (threadIdx.x & (kWave - 1)) * 4;
-    const uint8_t* c = which ? v : m;
-    O* out = which ? out_v : out_m;
-    if (!out) continue;
-    const float scale = scale_of((which ? sv : sm)[block]);
-    float o[4];
-    if (aligned && i + 4 <= n) {
-      const uint32_t codes = __builtin_nontemporal_load((const uint32_t*)(c + i));
-      if (which)
-        decode_v4(codes, scale, o);
-      else
-        decode_m4(codes, scale, o);
-      Vec<O, 4>::store(out + i, o);
+      for (int u = 0; u < 4; ++u) {
+        const int64_t i = e0 + u * 2048 + threadIdx.x * 8;
+        w[u] = stream_load8(codes + i);
+        s[u] = scales[i / kQuantBlock];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float lo[4], hi[4], o[8];
+        decode(w[u].x, scale_of(s[u]), lo);
+        decode(w[u].y, scale_of(s[u]), hi);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = lo[k], o[4 + k] = hi[k];
+        Vec<O, 8>::store(out + e0 + u * 2048 + threadIdx.x * 8, o);
+      }
     } else {
-      for (int k = 0; k < 4 && i + k < n; ++k) {
-        if (which)
-          decode_v4(c[i + k], scale, o);
-        else
-          decode_m4(c[i + k], scale, o);
-        Elem<O>::store(out + i + k, o[0]);
+      for (int u = 0; u < 4; ++u) {
+        const int64_t i = e0 + u * 2048 + threadIdx.x * 8;
+        if (i >= n) break;
+        const float scale = scale_of(scales[i / kQuantBlock]);
+        float o[4];
+        if (aligned && i + 8 <= n) {
+          const u32x2 w = stream_load8(codes + i);
+          decode(w.x, scale, o);
+          Vec<O, 4>::store(out + i, o);
+          decode(w.y, scale, o);
+          Vec<O, 4>::store(out + i + 4, o);
+          continue;
+        }
+        for (int k = 0; k < 8 && i + k < n; ++k) {
+          decode(codes[i + k], scale, o);
+          Elem<O>::store(out + i + k, o[0]);
+        }
       }
     }
   }
 }
 
-template <typename P, typename G, int BITS>
-static void launch_adamw(const AdamArgs& A, bool master, unsigned grid, hipStream_t s) {
-  if constexpr (!std::is_same<P, float>::value) {  // an fp32 parameter is its own master
-    if (master) {
-      hipLaunchKernelGGL((adamw_kernel<P, G, BITS, true>), dim3(grid), dim3(kAdamThreads), 0, s, A);
-      return;
+// One launch after another over the tensors of a checked call.
+template <typename P, typename G, int BITS, bool MASTER>
+static int launch_adamw(const AdamCommon& common, const struct unirl_adamw_tensor* tensors, int64_t n, hipStream_t s) {
+  using Args = AdamArgs<BITS, MASTER>;
+  constexpr size_t kState = BITS == 32 ? 4 : 1;
+  Args A;
+  memset(&A, 0, sizeof(A));
+  static_cast<AdamCommon&>(A) = common;
+  for (int64_t i = 0; i < n;) {
+    int k = 0;
+    int64_t grid = 0;
+    for (; i < n && k < Args::kTensors; ++i) {
+      const struct unirl_adamw_tensor& T = tensors[i];
+      if (T.numel == 0) continue;
+      const int64_t blocks = (T.numel + adam_chunk(BITS) - 1) / adam_chunk(BITS);
+      if (grid + blocks > kMaxGrid) break;  // the next launch takes it
+      const bool vectors = aligned_to(T.param, 4 * sizeof(P)) && aligned_to(T.grad, 4 * sizeof(G)) &&
+                           aligned_to(T.exp_avg, 4 * kState) && aligned_to(T.exp_avg_sq, 4 * kState) &&
+                           (!MASTER || aligned_to(T.master, 16));
+      auto& E = A.t[k];
+      E.param = T.param;
+      E.grad = T.grad;
+      E.exp_avg = T.exp_avg;
+      E.exp_avg_sq = T.exp_avg_sq;
+      E.numel2 = 2 * T.numel + vectors;
+      if constexpr (MASTER) E.master = T.master;
+      if constexpr (BITS == 8) {
+        E.exp_avg_scale = T.exp_avg_scale;
+        E.exp_avg_sq_scale = T.exp_avg_sq_scale;
+        E.index_base = T.index_base;
+      }
+      A.first[k++] = (uint32_t)grid;
+      grid += blocks;
     }
+    if (k == 0) break;
+    for (int j = k; j < Args::kTensors; ++j) A.first[j] = 0xffffffffu;
+    hipLaunchKernelGGL((adamw_kernel<P, G, BITS, MASTER>), dim3((unsigned)grid), dim3(kAdamThreads), 0, s, A);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL((adamw_kernel<P, G, BITS, false>), dim3(grid), dim3(kAdamThreads), 0, s, A);
+  return UNIRL_OK;
 }
 template <typename P, typename G>
-static void launch_adamw(const AdamArgs& A, int bits, bool master, unsigned grid, hipStream_t s) {
-  if (bits == 32)
-    launch_adamw<P, G, 32>(A, master, grid, s);
-  else
-    launch_adamw<P, G, 8>(A, master, grid, s);
+static int launch_adamw(const AdamCommon& c, const struct unirl_adamw_params* q, const struct unirl_adamw_tensor* t, int64_t n,
+                        hipStream_t s) {
+  if constexpr (!std::is_same<P, float>::value) {  // an fp32 parameter is its own master
+    if (q->use_master) return q->state_bits == 32 ? launch_adamw<P, G, 32, true>(c, t, n, s) : launch_adamw<P, G, 8, true>(c, t, n, s);
+  }
+  return q->state_bits == 32 ? launch_adamw<P, G, 32, false>(c, t, n, s) : launch_adamw<P, G, 8, false>(c, t, n, s);
 }
 
 }  // namespace unirl
@@ -569,9 +681,9 @@ extern "C" int unirl_adamw_step(const struct unirl_adamw_tensor* tensors, int64_
     if (!aligned_to(T.param, ps) || !aligned_to(T.grad, gs) || !aligned_to(T.exp_avg, ss) ||
         !aligned_to(T.exp_avg_sq, ss) || !aligned_to(T.master, 4))
       return UNIRL_E_ALIGN;
-    if (T.numel > kAdamChunk * kMaxGrid) return UNIRL_E_LIMIT;
+    if (T.numel > adam_chunk(q->state_bits) * kMaxGrid) return UNIRL_E_LIMIT;
   }
-  AdamArgs A;
+  AdamCommon A;
   memset(&A, 0, sizeof(A));
   A.control = (const AdamControl*)q->control;
   A.norm = q->max_norm >= 0.0f || q->skip_nonfinite ? q->grad_norm : nullptr;
@@ -587,41 +699,13 @@ extern "C" int unirl_adamw_step(const struct unirl_adamw_tensor* tensors, int64_
     const AdamScalars S = {q->lr, q->beta1, q->beta2, q->weight_decay, q->seed};
     A.host = control_of(S, q->step);
   }
-  for (int64_t i = 0; i < n_tensors;) {
-    int k = 0;
-    int64_t grid = 0;
-    A.aligned = 0;
-    for (; i < n_tensors && k < kAdamTensors; ++i) {
-      const struct unirl_adamw_tensor& T = tensors[i];
-      if (T.numel == 0) continue;
-      const int64_t blocks = (T.numel + kAdamChunk - 1) / kAdamChunk;
-      if (grid + blocks > kMaxGrid) break;  // the next launch takes it
-      A.t[k] = T;
-      A.first[k] = (uint32_t)grid;
-      if (aligned_to(T.param, 4 * ps) && aligned_to(T.grad, 4 * gs) && aligned_to(T.exp_avg, 4 * ss) &&
-          aligned_to(T.exp_avg_sq, 4 * ss) && aligned_to(T.master, 16))
-        A.aligned |= 1ull << k;
-      grid += blocks;
-      ++k;
-    }
-    if (k == 0) break;
-    for (int j = k; j < kAdamTensors; ++j) A.first[j] = 0xffffffffu;
-    hipStream_t s = (hipStream_t)stream;
-    const bool master = q->use_master != 0;
-    if (q->param_dtype == UNIRL_F32)
-      launch_adamw<float, float>(A, q->state_bits, false, (unsigned)grid, s);
-    else if (q->param_dtype == UNIRL_BF16 && q->grad_dtype == UNIRL_BF16)
-      launch_adamw<bf16_t, bf16_t>(A, q->state_bits, master, (unsigned)grid, s);
-    else if (q->param_dtype == UNIRL_BF16)
-      launch_adamw<bf16_t, float>(A, q->state_bits, master, (unsigned)grid, s);
-    else if (q->grad_dtype == UNIRL_F16)
-      launch_adamw<f16_t, f16_t>(A, q->state_bits, master, (unsigned)grid, s);
-    else
-      launch_adamw<f16_t, float>(A, q->state_bits, master, (unsigned)grid, s);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-  }
-  return UNIRL_OK;
+  hipStream_t s = (hipStream_t)stream;
+  if (q->param_dtype == UNIRL_F32) return launch_adamw<float, float>(A, q, tensors, n_tensors, s);
+  if (q->param_dtype == UNIRL_BF16)
+    return q->grad_dtype == UNIRL_BF16 ? launch_adamw<bf16_t, bf16_t>(A, q, tensors, n_tensors, s)
+                                       : launch_adamw<bf16_t, float>(A, q, tensors, n_tensors, s);
+  return q->grad_dtype == UNIRL_F16 ? launch_adamw<f16_t, f16_t>(A, q, tensors, n_tensors, s)
+                                    : launch_adamw<f16_t, float>(A, q, tensors, n_tensors, s);
 }
 
 extern "C" int unirl_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const uint8_t* exp_avg_scale,
@@ -634,12 +718,12 @@ extern "C" int unirl_adamw_moments(const void* exp_avg, const void* exp_avg_sq, 
     return UNIRL_E_NULL;
   const size_t os = dtype_size(out_dtype);
   if (!aligned_to(out_exp_avg, os) || !aligned_to(out_exp_avg_sq, os)) return UNIRL_E_ALIGN;
-  int64_t grid = (numel + 4 * kQuantBlock - 1) / (4 * kQuantBlock);
+  int64_t grid = (numel + kMomentsChunk - 1) / kMomentsChunk;
   if (grid > kMaxGrid) grid = kMaxGrid;
-  const int aligned = aligned_to(exp_avg, 4) && aligned_to(exp_avg_sq, 4) && aligned_to(out_exp_avg, 4 * os) &&
-                      aligned_to(out_exp_avg_sq, 4 * os);
+  const int aligned = aligned_to(exp_avg, 8) && aligned_to(exp_avg_sq, 8) && aligned_to(out_exp_avg, 16) &&
+                      aligned_to(out_exp_avg_sq, 16);
 #define UNIRL_MOMENTS(O)                                                                                            \
-  hipLaunchKernelGGL((adamw_moments_kernel<O>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream,            \
+  hipLaunchKernelGGL((adamw_moments_kernel<O>), dim3((unsigned)grid, 2), dim3(256), 0, (hipStream_t)stream,            \
                      (const uint8_t*)exp_avg, (const uint8_t*)exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, numel, \
                      (O*)out_exp_avg, (O*)out_exp_avg_sq, aligned)
   if (out_dtype == UNIRL_F32)

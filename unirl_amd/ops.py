@@ -1622,7 +1622,7 @@ def adamw_step(
     skip_nonfinite: bool = False,
     control: Optional[torch.Tensor] = None,
 ) -> None:
-    """One AdamW step (decoupled weight decay) over lists of tensors, in place, 48 tensors a launch::
+    """One AdamW step (decoupled weight decay) over lists of tensors, in place, 50 or more tensors a launch::
 
         m = b1 m + (1 - b1) c g;   v = b2 v + (1 - b2) (c g)^2
         p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
