@@ -336,6 +336,32 @@ def test_captured_forward_and_backward(dev):
                 assert torch.equal(o, e)
 
 
+@pytest.mark.parametrize("bias", [False, True])
+def test_backward_stays_inside_its_scratch(dev, bias):
+    """Scratch of exactly the documented size: the bytes behind it keep their values (and the entry point
+    itself refuses a launch whose partial rows would not fit)."""
+    import ctypes
+
+    from unirl_amd import _native as N
+    from unirl_amd import ops
+
+    for dtype in (torch.bfloat16, torch.float32):
+        for D in (8, 64, 100, 264, 513, 1024, 1536, 2048, 2304, 2560, 2568, 2600, 3200, 3333, 4096, 4608, 5120, 7168, 8192, 10240):
+            for G, R in ((1, 3000), (3, 1100)):
+                x = torch.randn(G * R, D, device=dev).to(dtype)
+                w = torch.ones(D, device=dev, dtype=dtype)
+                _, mean, rstd = ops.layer_norm(x, w, w, want_stats=True)
+                size = int(N.lib().unirl_layer_norm_bwd_scratch_bytes(G, R, D))
+                scratch = torch.full((size + 4096,), 77, dtype=torch.uint8, device=dev)
+                dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
+                desc = N.NormDesc(x=N.ptr(x), dtype=N.dtype_code(dtype), x_group_stride=R * D, x_row_stride=D, groups=G, rows=R, D=D,
+                                  gain=N.ptr(w), gain_dtype=N.dtype_code(dtype), center=1, mean=N.ptr(mean), rstd=N.ptr(rstd))
+                rc = N.lib().unirl_layer_norm_bwd(ctypes.byref(desc), N.ptr(x), R * D, D, N.ptr(dx), N.ptr(dw),
+                                                  N.ptr(db) if bias else None, 0, N.ptr(scratch), size, N.current_stream(dev))
+                assert rc == 0, (D, G, R, rc)
+                assert bool((scratch[size:] == 77).all()), (D, G, R)
+
+
 def test_rows_outside_a_view_stay_untouched_and_refusals(dev):
     from unirl_amd import models, ops
 

@@ -170,8 +170,8 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
 
 // Both kernels: a wavefront (or workgroup) walks over rows of one group with the gain in registers and
 // the next row on its way while it works on one.
-template <typename T, int VEC, int E, bool ONE_WAVE, bool BIAS>
-__global__ __launch_bounds__(ONE_WAVE ? kNormFwdRows * kWave : 1024) void norm_fwd_kernel(NormArgs A) {
+template <typename T, int VEC, int E, bool ONE_WAVE, bool BIAS, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormArgs A) {
   __shared__ float lds[16];
   const uint32_t tid = ONE_WAVE ? threadIdx.x & (kWave - 1) : threadIdx.x;
   const uint32_t step = (ONE_WAVE ? kWave : blockDim.x) * VEC;
@@ -228,8 +228,8 @@ __global__ __launch_bounds__(ONE_WAVE ? kNormFwdRows * kWave : 1024) void norm_f
 
 // The sums of the columns stay in registers as well; a workgroup leaves one partial row per sum, and
 // norm_param_kernel adds those in order.
-template <typename T, int VEC, int E, bool ONE_WAVE, bool BIAS>
-__global__ __launch_bounds__(ONE_WAVE ? kNormBwdRows * kWave : 1024) void norm_bwd_kernel(NormArgs A) {
+template <typename T, int VEC, int E, bool ONE_WAVE, bool BIAS, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormArgs A) {
   extern __shared__ float sums[];  // ONE_WAVE: 4 D floats to join the wavefronts; else 2 x 2 x 16 floats
   const uint32_t tid = ONE_WAVE ? threadIdx.x & (kWave - 1) : threadIdx.x;
   const uint32_t step = (ONE_WAVE ? kWave : blockDim.x) * VEC;
@@ -358,6 +358,163 @@ __global__ __launch_bounds__(ONE_WAVE ? kNormBwdRows * kWave : 1024) void norm_b
   }
 }
 
+// --- rows of at most 32 vectors (heads of 64 or 128): several rows share a wavefront ----------------
+// Sum over each group of LANES adjacent lanes (8, 16, 32), in every one of them: swaps inside quads, then
+// mirrored halves of 8 and 16 lanes (each lane of a quad, then of eight, holds the same sum by then).
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += __int_as_float(dpp_move<0xB1, 0xf>(0, __float_as_int(v)));   // lanes 1 0 3 2
+  v += __int_as_float(dpp_move<0x4E, 0xf>(0, __float_as_int(v)));   // lanes 2 3 0 1
+  v += __int_as_float(dpp_move<0x141, 0xf>(0, __float_as_int(v)));  // mirrored in 8
+  if constexpr (LANES >= 16) v += __int_as_float(dpp_move<0x140, 0xf>(0, __float_as_int(v)));  // mirrored in 16
+  if constexpr (LANES >= 32) v += __shfl_xor(v, 16);
+  return v;
+}
+
+// A wavefront takes 64 / LANES rows at a time; a lane keeps one vector of columns.  The descriptor
+// covers the rows that the wavefront reads, and a lane without a row or behind its end asks for an
+// offset outside it.
+constexpr uint32_t kOutside = 0x80000000u;
+template <typename T, int LANES>
+struct NarrowRows {
+  static constexpr int VEC = 16 / (int)sizeof(T), kRows = kWave / LANES;
+  uint32_t sub, col;
+  bool live;
+  __device__ __forceinline__ NarrowRows(uint32_t D) {
+    const uint32_t lane = threadIdx.x & (kWave - 1);
+    sub = lane / LANES;
+    col = lane % LANES * VEC;
+    live = col < D;
+  }
+  // rows [row, row + kRows) of a tensor whose rows are `stride` elements apart
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const T* base, int64_t row, int64_t stride) const {
+    return row_rsrc(base + row * stride, kOutside - 1);
+  }
+  __device__ __forceinline__ uint32_t off(int64_t row, int64_t rows, int64_t stride) const {
+    return live && row + sub < rows ? (sub * (uint32_t)stride + col) * (uint32_t)sizeof(T) : kOutside;
+  }
+};
+
+template <typename T, int LANES, bool BIAS>
+__global__ __launch_bounds__(256) void norm_narrow_fwd_kernel(NormArgs A) {
+  using N = NarrowRows<T, LANES>;
+  constexpr int VEC = N::VEC;
+  const N at(A.D);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t group = blockIdx.y, stride = (int64_t)gridDim.x * 4 * N::kRows;
+  const T* x = (const T*)A.x + group * A.x_group_stride;
+  int64_t row = ((int64_t)blockIdx.x * 4 + wave) * N::kRows;
+  if (row >= A.rows) return;
+  Packed<T, VEC, kStreaming> raw;
+  raw.load(at.rsrc(x, row, A.x_row_stride), at.off(row, A.rows, A.x_row_stride));
+  float w[VEC], b[BIAS ? VEC : 1];
+  load_param<VEC, VEC>(A.gain, A.gain_dtype, group * A.gain_group_stride, A.D, at.col, 0, 1.0f, A.gain_offset, w);
+  if constexpr (BIAS) load_param<VEC, VEC>(A.bias, A.gain_dtype, group * A.bias_group_stride, A.D, at.col, 0, 0.0f, 0.0f, b);
+  for (; row < A.rows; row += stride) {
+    float v[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = raw.get(k);
+    if (row + stride < A.rows)
+      raw.load(at.rsrc(x, row + stride, A.x_row_stride), at.off(row + stride, A.rows, A.x_row_stride));
+    float mean = 0.0f;
+    if (A.center) {
+      float s = 0.0f;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s += v[k];
+      mean = lanes_sum<LANES>(s) * A.inv_d;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[k] = at.live ? v[k] - mean : 0.0f;
+    }
+    float q = 0.0f;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) q = fmaf(v[k], v[k], q);
+    const float rstd = 1.0f / sqrtf(lanes_sum<LANES>(q) * A.inv_d + A.eps);
+    const int64_t flat = group * A.rows + row;
+    float o[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const float xh = v[k] * rstd;
+      o[k] = BIAS ? fmaf(xh, w[k], b[BIAS ? k : 0]) : xh * w[k];
+    }
+    store_vec<T, VEC>(at.rsrc((const T*)A.out + group * A.rows * A.D, row, A.D), at.off(row, A.rows, A.D), o);
+    if (at.col == 0 && row + at.sub < A.rows) {
+      if (A.mean) A.mean[flat + at.sub] = mean;
+      if (A.rstd) A.rstd[flat + at.sub] = rstd;
+    }
+  }
+}
+
+template <typename T, int LANES, bool BIAS>
+__global__ __launch_bounds__(512) void norm_narrow_bwd_kernel(NormArgs A) {
+  using N = NarrowRows<T, LANES>;
+  constexpr int VEC = N::VEC;
+  __shared__ float sums[512 * VEC];  // [wavefront * rows of one][LANES * VEC]
+  const N at(A.D);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t group = blockIdx.y, stride = (int64_t)gridDim.x * kNormBwdRows * N::kRows;
+  const T* x = (const T*)A.x + group * A.x_group_stride;
+  const T* dy = (const T*)A.dy + group * A.dy_group_stride;
+  int64_t row = ((int64_t)blockIdx.x * kNormBwdRows + wave) * N::kRows;
+  Packed<T, VEC, kStreaming> rx, rg;
+  float rstd = 0.0f, mean = 0.0f;
+  const auto load = [&](int64_t r) {
+    rx.load(at.rsrc(x, r, A.x_row_stride), at.off(r, A.rows, A.x_row_stride));
+    rg.load(at.rsrc(dy, r, A.dy_row_stride), at.off(r, A.rows, A.dy_row_stride));
+    const int64_t flat = group * A.rows + (r + at.sub < A.rows ? r + at.sub : A.rows - 1);
+    rstd = A.rstd[flat];
+    if (A.center) mean = A.mean[flat];
+  };
+  if (row < A.rows) load(row);
+  float w[VEC], dw[VEC], db[BIAS ? VEC : 1];
+  load_param<VEC, VEC>(A.gain, A.gain_dtype, group * A.gain_group_stride, A.D, at.col, 0, 1.0f, A.gain_offset, w);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) dw[k] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < (BIAS ? VEC : 1); ++k) db[k] = 0.0f;
+  for (; row < A.rows; row += stride) {
+    float xh[VEC], g[VEC];
+    const float s = rstd;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      xh[k] = (rx.get(k) - mean) * s;
+      g[k] = rg.get(k);
+    }
+    if (row + stride < A.rows) load(row + stride);
+    // behind the rows and their ends dy is 0, and with it every product below
+    float c1 = 0.0f, c2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      dw[k] = fmaf(g[k], xh[k], dw[k]);
+      if constexpr (BIAS) db[k] += g[k];
+      g[k] *= w[k];
+      c1 = fmaf(g[k], xh[k], c1);
+      c2 += g[k];
+    }
+    c1 = lanes_sum<LANES>(c1) * A.inv_d;
+    c2 = A.center ? lanes_sum<LANES>(c2) * A.inv_d : 0.0f;
+    if (A.out) {
+      float o[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) o[k] = (fmaf(-xh[k], c1, g[k]) - c2) * s;
+      store_vec<T, VEC>(at.rsrc((const T*)A.out + group * A.rows * A.D, row, A.D), at.off(row, A.rows, A.D), o);
+    }
+  }
+  if (!A.partial) return;
+#pragma unroll
+  for (int which = 0; which < (BIAS ? 2 : 1); ++which) {
+    if (which) __syncthreads();
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sums[threadIdx.x * VEC + k] = which ? db[BIAS ? k : 0] : dw[k];
+    __syncthreads();
+    float* out = A.partial + (which ? A.partial_bias : 0) + (group * gridDim.x + blockIdx.x) * A.D;
+    for (uint32_t c = threadIdx.x; c < A.D; c += 512) {
+      float v = 0.0f;
+      for (int h = 0; h < 512 / LANES; ++h) v += sums[h * (LANES * VEC) + c];
+      out[c] = v;
+    }
+  }
+}
+
 // out[set][c] = sum of `n` partial rows, in a fixed order: 32 columns x 32 slices of the rows a
 // workgroup, eight rows' loads of a lane in flight (a plain loop makes one trip to memory per row).
 // blockIdx.z: dgain, dbias.
@@ -391,38 +548,49 @@ __global__ __launch_bounds__(1024) void norm_param_kernel(const float* partial, 
 
 // --- shapes of launches -----------------------------------------------------
 struct NormShape {
-  bool one_wave;
+  int lanes;  // of one row: 8, 16, 32 or 64 of a wavefront, 0 = a workgroup
   int vec, elems, threads;
 };
-// Rows of up to 64 * 64 elements (forward) or 64 * 40 (backward, whose lanes hold five numbers per
-// element) belong to one wavefront (no barrier), longer ones to a workgroup of as many threads as
-// 8 elements each ask for, up to 1024.
-static NormShape norm_shape(int64_t D, int dtype, bool vectors, bool backward) {
+// Rows of up to 32 vectors share a wavefront.  Rows of up to 64 * 64 elements (forward) or 64 * 32
+// (backward, whose lanes hold five numbers per element; 64 * 40 in 16 bits without a bias, which still
+// fits the registers) belong to one wavefront, longer ones to a workgroup of as few elements a lane (8,
+// 16, 32) as 512 threads allow, since wider workgroups leave too few registers or too few of them
+// resident (backward, bf16 [13950, 7168]: 896 threads of 8 elements 229 us, 448 of 16 116 us).  Behind
+// 16384 elements 1024 threads spill in the backward (0.7 to 1.4 TB/s), which such rows have to bear.
+static NormShape norm_shape(int64_t D, int dtype, bool vectors, bool backward, bool bias) {
   NormShape S;
   S.vec = vectors ? 16 / (int)dtype_size(dtype) : 1;
-  S.one_wave = D <= kWave * (vectors ? (backward ? 40 : 64) : 32);
-  if (S.one_wave) {
+  const int64_t one_wave = !vectors ? 32 : (!backward ? 64 : (bias || dtype == UNIRL_F32 ? 32 : 40));
+  if (vectors && D <= 32 * S.vec) {
+    S.lanes = D <= 8 * S.vec ? 8 : (D <= 16 * S.vec ? 16 : 32);
+    S.elems = S.vec;
+    S.threads = kWave * (backward ? kNormBwdRows : kNormFwdRows);
+  } else if (D <= kWave * one_wave) {
+    S.lanes = 64;
     const int need = (int)((D + kWave - 1) / kWave);  // elements of a lane
     S.elems = need <= 8 ? 8 : (need <= 16 ? 16 : (need <= 32 && !vectors ? 32 : (need + 7) / 8 * 8));
     if (S.elems == 56) S.elems = 64;
     S.threads = kWave * (backward ? kNormBwdRows : kNormFwdRows);
   } else {
-    S.elems = D <= 1024 * 8 ? 8 : (D <= 1024 * 16 ? 16 : 32);
+    S.lanes = 0;
+    S.elems = D <= 512 * 8 ? 8 : (D <= 512 * 16 ? 16 : 32);
     S.threads = (int)((D + S.elems * kWave - 1) / (S.elems * kWave)) * kWave;
   }
   return S;
 }
-// Workgroups of one group.  Forward: up to 4 a compute unit.  Backward: as many as stay resident (16
-// wavefronts a compute unit for the narrower rows, 8 for those whose lanes need most of the registers)
-// with two rows a wavefront at least, since each leaves a partial row of D sums.
+// Workgroups of one group.  Forward: up to 4 a compute unit (8 where rows share a wavefront).
+// Backward: as many as stay resident, since a few more would run alone behind the others, with two rows
+// a wavefront at least, since each leaves a partial row of D sums.
 static int64_t norm_blocks(const NormShape& S, int64_t groups, int64_t rows, bool backward) {
-  const int64_t rows_at_once = S.one_wave ? S.threads / kWave : 1;
+  const int64_t rows_at_once = S.lanes ? S.threads / S.lanes : 1;
   const int64_t most = (rows + rows_at_once - 1) / rows_at_once;
-  int64_t total = kNormMaxBlocks;
+  int64_t total = S.lanes && S.lanes < kWave ? 2 * kNormMaxBlocks : kNormMaxBlocks;
   if (backward) {
-    total = S.elems <= 16 ? 4096 : 2048;
-    total = total / (S.threads / kWave);
-    if (total < 256) total = 256;
+    // wavefronts that a compute unit's registers hold (16 are enough where rows share a wavefront)
+    const int64_t slots = S.lanes && S.lanes < kWave ? 16 : S.vec > 1 ? (S.elems <= 8 ? 28 : (S.elems <= 16 ? 16 : 8)) : (S.elems <= 8 ? 20 : (S.elems <= 16 ? 12 : 8));
+    const int64_t resident = slots / (S.threads / kWave);
+    total = 256 * (resident > 1 ? resident : 1);
+    if (total > kNormMaxBlocks) total = kNormMaxBlocks;  // what unirl_layer_norm_bwd_scratch_bytes has room for
     const int64_t enough = (rows * groups + 2 * rows_at_once - 1) / (2 * rows_at_once);
     if (total > enough) total = enough;
   }
@@ -430,32 +598,58 @@ static int64_t norm_blocks(const NormShape& S, int64_t groups, int64_t rows, boo
   return want < most ? want : most;
 }
 
-template <typename T, int VEC, int E, bool ONE_WAVE, bool BIAS>
+template <typename T, int VEC, int E, bool BIAS>
 static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool backward, hipStream_t s) {
-  if (!backward) {
-    hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, ONE_WAVE, BIAS>), grid, dim3(S.threads), 0, s, A);
-  } else if constexpr (!ONE_WAVE || E <= 40) {
-    hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, ONE_WAVE, BIAS>), grid, dim3(S.threads),
-                       ONE_WAVE ? (size_t)A.D * (kNormBwdRows / 2 * 4) : 64 * 4, s, A);
+  const dim3 block(S.threads);
+  if (S.lanes == kWave) {
+    if (!backward)
+      hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, true, BIAS, kNormFwdRows * kWave>), grid, block, 0, s, A);
+    else if constexpr (E <= 32 || (E == 40 && sizeof(T) == 2 && !BIAS))
+      hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, true, BIAS, kNormBwdRows * kWave>), grid, block,
+                         (size_t)A.D * (kNormBwdRows / 2 * 4), s, A);
+  } else if constexpr (E == 8 || E == 16 || E == 32) {
+    constexpr size_t kSlots = 64 * 4;
+    if (S.threads <= 512) {
+      if (backward)
+        hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, BIAS, 512>), grid, block, kSlots, s, A);
+      else
+        hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, false, BIAS, 512>), grid, block, 0, s, A);
+    } else if constexpr (E == 32) {
+      if (backward)
+        hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, BIAS, 1024>), grid, block, kSlots, s, A);
+      else
+        hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, false, BIAS, 1024>), grid, block, 0, s, A);
+    }
   }
 }
 template <typename T, int VEC, int E>
 static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool backward, bool bias, hipStream_t s) {
-  if (S.one_wave) {
-    if (bias)
-      launch_norm<T, VEC, E, true, true>(A, S, grid, backward, s);
-    else
-      launch_norm<T, VEC, E, true, false>(A, S, grid, backward, s);
-  } else if constexpr (E == 8 || E == 16 || E == 32) {
-    if (bias)
-      launch_norm<T, VEC, E, false, true>(A, S, grid, backward, s);
-    else
-      launch_norm<T, VEC, E, false, false>(A, S, grid, backward, s);
-  }
+  if (bias)
+    launch_norm<T, VEC, E, true>(A, S, grid, backward, s);
+  else
+    launch_norm<T, VEC, E, false>(A, S, grid, backward, s);
+}
+template <typename T, int LANES>
+static void launch_narrow(const NormArgs& A, const NormShape& S, dim3 grid, bool backward, bool bias, hipStream_t s) {
+  const dim3 block(S.threads);
+  if (backward && bias)
+    hipLaunchKernelGGL((norm_narrow_bwd_kernel<T, LANES, true>), grid, block, 0, s, A);
+  else if (backward)
+    hipLaunchKernelGGL((norm_narrow_bwd_kernel<T, LANES, false>), grid, block, 0, s, A);
+  else if (bias)
+    hipLaunchKernelGGL((norm_narrow_fwd_kernel<T, LANES, true>), grid, block, 0, s, A);
+  else
+    hipLaunchKernelGGL((norm_narrow_fwd_kernel<T, LANES, false>), grid, block, 0, s, A);
 }
 template <typename T>
 static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool backward, bool bias, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
+  switch (S.lanes) {
+    case 8: return launch_narrow<T, 8>(A, S, grid, backward, bias, s);
+    case 16: return launch_narrow<T, 16>(A, S, grid, backward, bias, s);
+    case 32: return launch_narrow<T, 32>(A, S, grid, backward, bias, s);
+    default: break;
+  }
   if (S.vec == 1) {
     switch (S.elems) {
       case 8: return launch_norm<T, 1, 8>(A, S, grid, backward, bias, s);
@@ -483,10 +677,11 @@ static void launch_norm(const NormArgs& A, const NormShape& S, int dtype, dim3 g
     launch_norm<f16_t>(A, S, grid, backward, bias, s);
 }
 
-// Pointer and strides of a [groups, rows, D] operand suit 16-byte accesses.
+// Pointer and strides of a [groups, rows, D] operand suit 16-byte accesses (and the 32-bit offsets of
+// eight rows that share a wavefront).
 static bool vectors_ok(const void* p, int64_t gs, int64_t rs, int64_t D, int64_t groups, int64_t rows, size_t esize) {
   const int64_t v = 16 / (int64_t)esize;
-  return aligned_to(p, 16) && D % v == 0 && (rows < 2 || rs % v == 0) && (groups < 2 || gs % v == 0);
+  return aligned_to(p, 16) && D % v == 0 && (rows < 2 || (rs % v == 0 && rs < (1 << 24))) && (groups < 2 || gs % v == 0);
 }
 
 static bool params_vectors_ok(const struct unirl_norm_desc* d) {
@@ -547,7 +742,7 @@ extern "C" int unirl_layer_norm_fwd(const struct unirl_norm_desc* d, void* y, vo
   if (!aligned_to(y, es)) return UNIRL_E_ALIGN;
   const bool vectors = vectors_ok(d->x, d->x_group_stride, d->x_row_stride, d->D, d->groups, d->rows, es) &&
                        params_vectors_ok(d) && aligned_to(y, 16);
-  const NormShape S = norm_shape(d->D, d->dtype, vectors, false);
+  const NormShape S = norm_shape(d->D, d->dtype, vectors, false, d->bias != nullptr);
   for (int64_t g0 = 0; g0 < d->groups; g0 += kNormMaxGroups) {
     const int64_t ng = d->groups - g0 < kNormMaxGroups ? d->groups - g0 : kNormMaxGroups;
     NormArgs A = norm_args(d, g0);
@@ -589,11 +784,13 @@ extern "C" int unirl_layer_norm_bwd(const struct unirl_norm_desc* d, const void*
     if (!aligned_to(dy, es) || !aligned_to(dx, es)) return UNIRL_E_ALIGN;
     const bool vectors = vectors_ok(d->x, d->x_group_stride, d->x_row_stride, d->D, d->groups, d->rows, es) &&
                          vectors_ok(dy, dy_group_stride, dy_row_stride, d->D, d->groups, d->rows, es) && params_vectors_ok(d) && aligned_to(dx, 16);
-    const NormShape S = norm_shape(d->D, d->dtype, vectors, true);
+    const NormShape S = norm_shape(d->D, d->dtype, vectors, true, dbias != nullptr);
     blocks = norm_blocks(S, d->groups, d->rows, true);
     if (params) {
       if (!scratch || scratch_bytes < unirl_layer_norm_bwd_scratch_bytes(d->groups, d->rows, d->D)) return UNIRL_E_WORKSPACE;
       if (!aligned_to(scratch, 16)) return UNIRL_E_ALIGN;
+      // the launch's own partial rows, whatever the function above says
+      if ((size_t)(d->groups * blocks * d->D) * (dbias ? 2 : 1) * sizeof(float) > scratch_bytes) return UNIRL_E_WORKSPACE;
     }
     if (!params && !dx) return UNIRL_OK;
     part_bias = d->groups * blocks * d->D;
