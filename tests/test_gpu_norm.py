@@ -394,6 +394,7 @@ def test_replay_log_prob_behind_a_final_norm(dev):
     """chunked_replay_logp(final_norm=...) on hidden states from before the norm: the same log-probs and
     gradients as the norm called in front of it, and the gain's gradient."""
     from unirl_amd import models
+    from unirl_amd.models.ar_logp import _apply_final_norm
 
     g = torch.Generator().manual_seed(9)
     hidden = torch.randn(2, 21, 128, generator=g).bfloat16().to(dev)
@@ -409,7 +410,7 @@ def test_replay_log_prob_behind_a_final_norm(dev):
         if isinstance(norm, torch.nn.LayerNorm):
             y = models.layer_norm(h[:, :20], norm.weight, norm.bias, norm.eps)
         else:
-            y = models.rms_norm(h[:, :20], norm.weight, norm.eps or torch.finfo(torch.bfloat16).eps)
+            y = models.rms_norm(h[:, :20], norm.weight, norm.eps or torch.finfo(torch.float32).eps)
         plain = models.chunked_replay_logp(head, y, tokens, 0.9)
         assert torch.equal(out, plain)
         for a, b in zip(got, torch.autograd.grad(plain.sum(), leaves)):
@@ -418,6 +419,12 @@ def test_replay_log_prob_behind_a_final_norm(dev):
         with torch.no_grad():
             scored = models.chunked_replay_logp(head, h, tokens, 0.9, final_norm=norm)
             assert torch.equal(scored, models.chunked_replay_logp(head, y.detach(), tokens, 0.9))
+    # small states, where the module's default eps counts: two roundings to bf16 apart from the module at most
+    small = (torch.randn(2, 20, 128, generator=g) * 2e-3).bfloat16().to(dev)
+    for norm in (torch.nn.RMSNorm(128), torch.nn.LayerNorm(128)):
+        norm = norm.to(dev, torch.bfloat16)
+        got = _apply_final_norm(norm, small).float()
+        assert bool(((got - norm(small).float()).abs() <= 2 * 2.0**-8 * 1.01 * got.abs() + 1e-6).all())
     called = []
 
     def other(t):

@@ -574,6 +574,36 @@ def test_optimizer_state_round_trip(dev, bits, capturable):
         other.load_state_dict(a.state_dict())
 
 
+def test_optimizer_copies_groups_and_schedulers(dev):
+    """A deep copy steps like the original; a scheduler's rate is used; a group added later joins in."""
+    import copy
+
+    from unirl_amd.train import AdamW
+
+    ours = model(torch.float32, dev)
+    a = AdamW(ours[:2], lr=1e-2, state_bits=8, max_grad_norm=1.0, capturable=True, skip_nonfinite=True)
+    rate = torch.optim.lr_scheduler.LambdaLR(a, lambda k: 1.0 / (k + 1))
+    set_grads(ours, 0)
+    a.step()
+    rate.step()
+    a.add_param_group(dict(params=ours[2:], state_bits=32))
+    set_grads(ours, 1)
+    a.step()
+    twin = copy.deepcopy({"opt": a, "params": ours})
+    b, theirs = twin["opt"], twin["params"]
+    assert (b.max_grad_norm, b.skip_nonfinite, b.capturable) == (1.0, True, True)
+    set_grads(ours, 2)
+    set_grads(theirs, 2)
+    before = [p.detach().clone() for p in ours]
+    a.step()
+    b.step()
+    for p, q, old in zip(ours, theirs, before):
+        assert torch.equal(p, q) and not torch.equal(p, old)
+    assert [int(g["step"]) for g in b.param_groups] == [3, 2]
+    bases = [a.state[p]["index_base"] for p in ours]
+    assert len(set(bases)) == len(bases) and all(x % 256 == 0 for x in bases)
+
+
 def test_master_weights_keep_small_updates(dev):
     """Updates of a fiftieth of a bf16 unit: 100 of them move the parameter with a master, none without."""
     from unirl_amd.train import AdamW
@@ -624,19 +654,19 @@ def test_captured_optimizer(dev):
 
 
 def test_policy_update_end_to_end(dev):
-    """Final norm, head, log-prob, GRPO loss with its gradient, global norm and clipped step in one run, against the
-    same chain in 64 bits on the CPU; the bf16 chain's gradients are compared at bf16's resolution of
+    """Final norm, head, log-prob, GRPO loss with its gradient (at ratio 1, where it is the policy gradient), global
+    norm and clipped step in one run, against the same chain in 64 bits on the CPU; the bf16 chain's gradients are compared at bf16's resolution of
     their largest terms (2^-7 of the column's largest: logits, norm output and gradient are rounded to
     2^-8 each), the step with the chain's own gradients at the step's bounds."""
     from unirl_amd import models
-    from unirl_amd.algorithms import fused_token_loss_backward  # noqa: F401  (the loss the chain stands for)
+    from unirl_amd.algorithms import fused_token_loss_backward
     from unirl_amd.train import AdamW
 
     g = torch.Generator().manual_seed(1)
     B, T, D, V = 4, 48, 128, 512
     hidden = torch.randn(B, T, D, generator=g).bfloat16()
     tokens = torch.randint(0, V, (B, T), generator=g)
-    adv = torch.randn(B, T, generator=g)
+    adv = torch.randn(B, generator=g)
     norm = torch.nn.RMSNorm(D, eps=1e-6, dtype=torch.bfloat16)
     head = torch.nn.Linear(D, V, bias=False, dtype=torch.bfloat16)
     with torch.no_grad():
@@ -646,13 +676,14 @@ def test_policy_update_end_to_end(dev):
     X = hidden.double()
     Y = X / torch.sqrt((X * X).mean(-1, keepdim=True) + 1e-6) * N
     logp = torch.log_softmax(Y @ W.t(), -1).gather(-1, tokens[..., None])[..., 0]
-    exact = torch.autograd.grad(-(logp * adv).mean(), [W, N])
+    exact = torch.autograd.grad(-(logp * adv[:, None]).mean(), [W, N])
 
     norm, head = norm.to(dev), head.to(dev)
     params = [head.weight, norm.weight]
     opt = AdamW(params, lr=1e-3, state_bits=8, master_weights=True, max_grad_norm=1e-3)
     new = models.chunked_replay_logp(head, hidden.to(dev), tokens.to(dev), final_norm=norm)
-    (-(new * adv.to(dev)).mean()).backward()
+    fused_token_loss_backward("grpo", new, new.detach(), adv.to(dev), loss_scale=1.0,
+                              lengths=torch.full((B,), T, device=dev, dtype=torch.int64))
     for p, e in zip(params, exact):
         off = (p.grad.double().cpu() - e).abs().max()
         assert float(off) <= 2.0**-7 * float(e.abs().max()), float(off / e.abs().max())

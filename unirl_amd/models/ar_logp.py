@@ -266,13 +266,14 @@ def _apply_final_norm(norm: Callable[[torch.Tensor], torch.Tensor], hidden: torc
                  or _m._global_backward_pre_hooks)
         and tuple(norm.normalized_shape) == (hidden.shape[-1],) and hidden.shape[-1] <= ops.NORM_MAX_DIM
         and hidden.is_cuda and hidden.dtype in _KERNEL_DTYPES and not torch.is_autocast_enabled("cuda")
-        and all(p.dtype in _KERNEL_DTYPES and p.device == hidden.device for p in norm.parameters())
+        and all(p.dtype == hidden.dtype and p.device == hidden.device for p in norm.parameters())
     )
     if not own:
         return norm(hidden)
     if kind is torch.nn.LayerNorm:
         return layer_norm(hidden, norm.weight, norm.bias, norm.eps)
-    return rms_norm(hidden, norm.weight, torch.finfo(hidden.dtype).eps if norm.eps is None else norm.eps)
+    # without an eps of its own nn.RMSNorm adds fp32's, also to 16-bit states (it computes in fp32)
+    return rms_norm(hidden, norm.weight, torch.finfo(torch.float32).eps if norm.eps is None else norm.eps)
 
 
 #: all of a replay's logits are kept for the backward (no second ``lm_head`` pass) up to this size

@@ -81,6 +81,17 @@ class AdamW(torch.optim.Optimizer):
             if not p.is_contiguous():
                 raise ValueError(f"parameters must be contiguous; got strides {p.stride()} of {tuple(p.shape)}")
 
+    # -- copies and pickles: the base class keeps defaults, state and groups alone ---------------------
+    _OPTIONS = ("max_grad_norm", "skip_nonfinite", "capturable", "_next_base")
+
+    def __getstate__(self) -> Dict[str, Any]:
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in self._OPTIONS}}
+
+    def __setstate__(self, state: Dict[str, Any]) -> None:
+        super().__setstate__(state)
+        self._controls = {}
+        self.grad_norm = None
+
     # -- state -------------------------------------------------------------
     def _new_state(self, group: Dict[str, Any], p: torch.Tensor) -> Dict[str, Any]:
         N.require_device(p, "parameter")
@@ -123,7 +134,6 @@ class AdamW(torch.optim.Optimizer):
                     f"{tuple(p.shape)}"
                 )
         super().load_state_dict(state_dict)
-        self._controls.clear()
         self._next_base = 0
         for p, i in zip(ours, ids):
             s = saved.get(i)
