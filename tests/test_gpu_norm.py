@@ -263,6 +263,24 @@ def test_constant_rows_large_values_and_bad_ones(dev):
     assert torch.isnan(y[2, 7]) and not y[2, :7].any() and torch.isnan(y[3]).all() and not y[5].any()
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 256), (torch.float32, 8), (torch.float32, 2048), (torch.float32, 8192),
+                                     (torch.bfloat16, 32), (torch.bfloat16, 256), (torch.bfloat16, 1024), (torch.float32, 1)])
+def test_gradient_of_large_constant_rows(dev, dtype, D):
+    """Rows of 2^123: the mean is exact (D is a power of two), the variance 0 and rstd 1 / sqrt(eps); lanes behind
+    the row's end must not bring in (0 - mean) rstd, which overflows.  dx = (a - mean(a)) / sqrt(eps)."""
+    x = torch.full((5, D), 2.0**123).to(dtype)
+    _, w, b, dy = make((5, D), dtype, D, False)
+    got = run(x, w, b, dy, 2.0**-18, "layer", dev)
+    a = dy.double() * w.double()
+    want = (a - a.mean(-1, keepdim=True)) * 2.0**9
+    # products and sums of a as in the module's comment, scaled by rstd; the value rounded to dtype
+    bound = 512 * U * (6 * a.abs() + 60 * a.abs().mean(-1, keepdim=True)) + half(dtype) * want.abs() * 1.01 + 1e-30
+    check(got["dx"], (want, bound), "dx")
+    assert not got["dw"].any()
+    check(got["db"], (dy.double().sum(0), 8 * U * dy.double().abs().sum(0) + half(dtype) * dy.double().sum(0).abs() * 1.01 + 1e-30),
+          "db")
+
+
 def test_gradient_against_differences(dev):
     """<dx, d> from the kernel against (f(x + t d) - f(x - t d)) / 2t of the 64-bit formula, t = 2^-20: the
     difference's own error is t^2 times the third derivative (below 1e-9 here) plus 2^-52 |f| / t."""

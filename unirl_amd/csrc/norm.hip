@@ -196,8 +196,8 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormArgs A) {
     if (A.center) {
       float s = 0.0f;
 #pragma unroll
-      for (int k = 0; k < E; ++k) s += v[k];
-      mean = row_sum<ONE_WAVE>(s, lds) * A.inv_d;
+      for (int k = 0; k < E; ++k) s = fmaf(v[k], A.inv_d, s);  // the sum itself could overflow
+      mean = row_sum<ONE_WAVE>(s, lds);
 #pragma unroll
       for (int j = 0; j < E / VEC; ++j)
 #pragma unroll
@@ -266,11 +266,16 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormArgs A) {
       rx.load(x + (row + stride) * A.x_row_stride, A.D, col, step);
       rg.load(dy + (row + stride) * A.dy_row_stride, A.D, col, step);
     }
-    // behind the row's end dy is 0, and with it every product below
+    // behind the row's end x and dy are 0, and so is xh there (0 - mean could overflow on its way)
+#pragma unroll
+    for (int j = 0; j < E / VEC; ++j) {
+      const float mu = col + j * step < A.D ? mean : 0.0f;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) xh[j * VEC + k] = (xh[j * VEC + k] - mu) * rstd;
+    }
     float c1 = 0.0f, c2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-      xh[k] = (xh[k] - mean) * rstd;
       dw[k] = fmaf(g[k], xh[k], dw[k]);
       if constexpr (BIAS) db[k] += g[k];
       g[k] *= w[k];
@@ -420,8 +425,8 @@ __global__ __launch_bounds__(256) void norm_narrow_fwd_kernel(NormArgs A) {
     if (A.center) {
       float s = 0.0f;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) s += v[k];
-      mean = lanes_sum<LANES>(s) * A.inv_d;
+      for (int k = 0; k < VEC; ++k) s = fmaf(v[k], A.inv_d, s);  // the sum itself could overflow
+      mean = lanes_sum<LANES>(s);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) v[k] = at.live ? v[k] - mean : 0.0f;
     }
@@ -473,14 +478,14 @@ __global__ __launch_bounds__(512) void norm_narrow_bwd_kernel(NormArgs A) {
   for (int k = 0; k < (BIAS ? VEC : 1); ++k) db[k] = 0.0f;
   for (; row < A.rows; row += stride) {
     float xh[VEC], g[VEC];
-    const float s = rstd;
+    // behind the rows and their ends x and dy are 0, and so is xh there (0 - mean could overflow on its way)
+    const float s = rstd, mu = at.live && row + at.sub < A.rows ? mean : 0.0f;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      xh[k] = (rx.get(k) - mean) * s;
+      xh[k] = (rx.get(k) - mu) * s;
       g[k] = rg.get(k);
     }
     if (row + stride < A.rows) load(row + stride);
-    // behind the rows and their ends dy is 0, and with it every product below
     float c1 = 0.0f, c2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
@@ -587,7 +592,9 @@ static int64_t norm_blocks(const NormShape& S, int64_t groups, int64_t rows, boo
   int64_t total = S.lanes && S.lanes < kWave ? 2 * kNormMaxBlocks : kNormMaxBlocks;
   if (backward) {
     // wavefronts that a compute unit's registers hold (16 are enough where rows share a wavefront)
-    const int64_t slots = S.lanes && S.lanes < kWave ? 16 : S.vec > 1 ? (S.elems <= 8 ? 28 : (S.elems <= 16 ? 16 : 8)) : (S.elems <= 8 ? 20 : (S.elems <= 16 ? 12 : 8));
+    int64_t slots = S.elems <= 8 ? 28 : (S.elems <= 16 ? 16 : 8);
+    if (S.vec == 1) slots = S.elems <= 8 ? 20 : (S.elems <= 16 ? 12 : 8);
+    if (S.lanes && S.lanes < kWave) slots = 16;
     const int64_t resident = slots / (S.threads / kWave);
     total = 256 * (resident > 1 ? resident : 1);
     if (total > kNormMaxBlocks) total = kNormMaxBlocks;  // what unirl_layer_norm_bwd_scratch_bytes has room for
