@@ -556,16 +556,17 @@ struct NormShape {
   int lanes;  // of one row: 8, 16, 32 or 64 of a wavefront, 0 = a workgroup
   int vec, elems, threads;
 };
-// Rows of up to 32 vectors share a wavefront.  Rows of up to 64 * 64 elements (forward) or 64 * 32
-// (backward, whose lanes hold five numbers per element; 64 * 40 in 16 bits without a bias, which still
-// fits the registers) belong to one wavefront, longer ones to a workgroup of as few elements a lane (8,
-// 16, 32) as 512 threads allow, since wider workgroups leave too few registers or too few of them
-// resident (backward, bf16 [13950, 7168]: 896 threads of 8 elements 229 us, 448 of 16 116 us).  Behind
-// 16384 elements 1024 threads spill in the backward (0.7 to 1.4 TB/s), which such rows have to bear.
-static NormShape norm_shape(int64_t D, int dtype, bool vectors, bool backward, bool bias) {
+// Rows of up to 32 vectors share a wavefront (forward, bf16 [781250, 128]: 76 us, one row a wavefront 183).
+// Rows of up to 64 * 64 elements (forward) or 64 * 32 (backward, whose lanes hold five numbers per
+// element: 40 spill with a bias and gain nothing without, 27.5 and 27.1 us for bf16 [8192, 2560]) belong to one
+// wavefront, longer ones to a workgroup of as few elements a lane (8, 16, 32) as 512 threads allow,
+// since wider workgroups leave too few registers or too few of them resident (backward, bf16
+// [13950, 7168]: 896 threads of 8 elements 229 us, 448 of 16 116 us).  Behind 16384 elements 1024 threads
+// spill in the backward (0.7 to 1.4 TB/s), which such rows have to bear.
+static NormShape norm_shape(int64_t D, int dtype, bool vectors, bool backward) {
   NormShape S;
   S.vec = vectors ? 16 / (int)dtype_size(dtype) : 1;
-  const int64_t one_wave = !vectors ? 32 : (!backward ? 64 : (bias || dtype == UNIRL_F32 ? 32 : 40));
+  const int64_t one_wave = vectors && !backward ? 64 : 32;
   if (vectors && D <= 32 * S.vec) {
     S.lanes = D <= 8 * S.vec ? 8 : (D <= 16 * S.vec ? 16 : 32);
     S.elems = S.vec;
@@ -611,7 +612,7 @@ static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool b
   if (S.lanes == kWave) {
     if (!backward)
       hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, true, BIAS, kNormFwdRows * kWave>), grid, block, 0, s, A);
-    else if constexpr (E <= 32 || (E == 40 && sizeof(T) == 2 && !BIAS))
+    else if constexpr (E <= 32)
       hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, true, BIAS, kNormBwdRows * kWave>), grid, block,
                          (size_t)A.D * (kNormBwdRows / 2 * 4), s, A);
   } else if constexpr (E == 8 || E == 16 || E == 32) {
@@ -749,7 +750,7 @@ extern "C" int unirl_layer_norm_fwd(const struct unirl_norm_desc* d, void* y, vo
   if (!aligned_to(y, es)) return UNIRL_E_ALIGN;
   const bool vectors = vectors_ok(d->x, d->x_group_stride, d->x_row_stride, d->D, d->groups, d->rows, es) &&
                        params_vectors_ok(d) && aligned_to(y, 16);
-  const NormShape S = norm_shape(d->D, d->dtype, vectors, false, d->bias != nullptr);
+  const NormShape S = norm_shape(d->D, d->dtype, vectors, false);
   for (int64_t g0 = 0; g0 < d->groups; g0 += kNormMaxGroups) {
     const int64_t ng = d->groups - g0 < kNormMaxGroups ? d->groups - g0 : kNormMaxGroups;
     NormArgs A = norm_args(d, g0);
@@ -791,7 +792,7 @@ extern "C" int unirl_layer_norm_bwd(const struct unirl_norm_desc* d, const void*
     if (!aligned_to(dy, es) || !aligned_to(dx, es)) return UNIRL_E_ALIGN;
     const bool vectors = vectors_ok(d->x, d->x_group_stride, d->x_row_stride, d->D, d->groups, d->rows, es) &&
                          vectors_ok(dy, dy_group_stride, dy_row_stride, d->D, d->groups, d->rows, es) && params_vectors_ok(d) && aligned_to(dx, 16);
-    const NormShape S = norm_shape(d->D, d->dtype, vectors, true, dbias != nullptr);
+    const NormShape S = norm_shape(d->D, d->dtype, vectors, true);
     blocks = norm_blocks(S, d->groups, d->rows, true);
     if (params) {
       if (!scratch || scratch_bytes < unirl_layer_norm_bwd_scratch_bytes(d->groups, d->rows, d->D)) return UNIRL_E_WORKSPACE;

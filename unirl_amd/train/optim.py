@@ -154,50 +154,49 @@ class AdamW(torch.optim.Optimizer):
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         if capturing and not self.capturable:
             raise RuntimeError("AdamW: a captured step needs capturable=True (the count of steps would not move)")
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.grad is not None and p.grad.layout is not torch.strided:
-                    raise RuntimeError("AdamW does not support sparse gradients")
-        grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+        strided, state_of = torch.strided, self.state
+        pairs = [[(p, p.grad) for p in group["params"] if p.grad is not None] for group in self.param_groups]
+        if any(g.layout is not strided for group in pairs for _, g in group):
+            raise RuntimeError("AdamW does not support sparse gradients")
         self.grad_norm = None
-        if grads and (self.max_grad_norm is not None or self.skip_nonfinite):
-            self.grad_norm = ops.grad_norm(grads)
-        clip = dict(grad_norm=self.grad_norm, max_norm=self.max_grad_norm, skip_nonfinite=self.skip_nonfinite)
-        if self.grad_norm is None:
-            clip = {}
-        for index, group in enumerate(self.param_groups):
-            with_grad = [p for p in group["params"] if p.grad is not None]
+        clip: Dict[str, Any] = {}
+        if self.max_grad_norm is not None or self.skip_nonfinite:
+            grads = [g for group in pairs for _, g in group]
+            if grads:
+                self.grad_norm = ops.grad_norm(grads)
+                clip = dict(grad_norm=self.grad_norm, max_norm=self.max_grad_norm, skip_nonfinite=self.skip_nonfinite)
+        for index, (group, with_grad) in enumerate(zip(self.param_groups, pairs)):
             if not with_grad:
                 continue
-            for p in with_grad:
-                if not self.state[p]:
-                    self.state[p].update(self._new_state(group, p))
+            buckets: Dict[Any, List[Any]] = {}  # what shares a call: types, master, count of steps
+            counted = not self.capturable
+            for p, g in with_grad:
+                s = state_of[p]
+                if not s:
+                    s.update(self._new_state(group, p))
+                buckets.setdefault((p.dtype, g.dtype, "master" in s, s["step"]), []).append((p, g, s))
             how: Dict[str, Any] = {}
             if self.capturable:
-                how["control"] = self._advance(index, group, with_grad[0].device, clip)
+                how["control"] = self._advance(index, group, with_grad[0][0].device, clip)
             else:
                 how.update(lr=float(group["lr"]), weight_decay=group["weight_decay"], seed=group["seed"], **clip)
-            buckets: Dict[Any, List[torch.Tensor]] = {}
-            for p in with_grad:
-                s = self.state[p]
-                if not self.capturable:
-                    s["step"] += 1
-                buckets.setdefault((p.dtype, p.grad.dtype, "master" in s, s["step"]), []).append(p)
-            for (_, _, master, count), ps in buckets.items():
-                states = [self.state[p] for p in ps]
+            small = group["state_bits"] == 8
+            for (_, _, master, count), rows in buckets.items():
+                ps, gs, states = zip(*rows)
 
-                def column(name):
-                    return [s[name] for s in states]
+                def column(name, wanted=True):
+                    return [s[name] for s in states] if wanted else None
 
-                if not self.capturable:
-                    how["step"] = count
+                if counted:
+                    how["step"] = count + 1
                 ops.adamw_step(
-                    ps, [p.grad for p in ps], column("exp_avg"), column("exp_avg_sq"), betas=group["betas"], eps=group["eps"],
-                    masters=column("master") if master else None,
-                    exp_avg_scales=column("exp_avg_scale") if group["state_bits"] == 8 else None,
-                    exp_avg_sq_scales=column("exp_avg_sq_scale") if group["state_bits"] == 8 else None,
-                    index_bases=column("index_base"), **how,
+                    ps, gs, column("exp_avg"), column("exp_avg_sq"), betas=group["betas"], eps=group["eps"],
+                    masters=column("master", master), exp_avg_scales=column("exp_avg_scale", small),
+                    exp_avg_sq_scales=column("exp_avg_sq_scale", small), index_bases=column("index_base"), **how,
                 )
+                if counted:
+                    for s in states:
+                        s["step"] = count + 1
         return loss
 
     def _advance(self, index: int, group: Dict[str, Any], device: torch.device, clip: Dict[str, Any]) -> torch.Tensor:
