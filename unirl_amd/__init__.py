@@ -6,7 +6,8 @@ reference's call signatures:
 
     unirl_amd.sde          StepStrategy.denoise, Flow/Dance/CPS strategies, sigma schedule
     unirl_amd.algorithms   _grpo_clip_loss, _drpo_loss, _flowdppo_kl_adv_loss, GRPO, DRPO, ...
-    unirl_amd.models       token log-prob / entropy over the vocabulary
+    unirl_amd.models       token log-prob / entropy over the vocabulary, norms in front of a policy's output
+    unirl_amd.train        the optimizer step: gradient norm, AdamW with 32- or 8-bit moments
     unirl_amd.types        group-normalised advantages
     unirl_amd.ops          tensor-level wrappers of the raw entry points
 
