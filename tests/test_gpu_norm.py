@@ -408,6 +408,71 @@ def test_rows_outside_a_view_stay_untouched_and_refusals(dev):
         torch.autograd.grad(gx.sum(), x)
 
 
+def test_autograd_asks_for_what_it_needs(dev):
+    """Every choice of inputs that want a gradient, twice through one graph; an input written between
+    forward and backward is noticed; checkpointing recomputes the node."""
+    from torch.utils.checkpoint import checkpoint
+
+    from unirl_amd import models
+
+    x, w, b, dy = make((33, 136), torch.bfloat16, 21, False)
+    want = reference(x, w, b, dy, 1e-5, False, 0.0)
+    for mask in range(1, 8):
+        leaves = [t.to(dev).requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((x, w, b))]
+        y = models.layer_norm(*leaves)
+        asked = [(n, t) for n, t in zip(("dx", "dw", "db"), leaves) if t.requires_grad]
+        for keep in (True, False):
+            grads = torch.autograd.grad(y, [t for _, t in asked], dy.to(dev), retain_graph=keep)
+            for (name, _), g in zip(asked, grads):
+                check(g, want[name], f"{name} of mask {mask}")
+        with torch.no_grad():
+            assert not models.layer_norm(*leaves).requires_grad
+    for i in range(2):  # x and the gain are read again by the backward
+        leaves = [t.to(dev).requires_grad_(True) for t in (x, w, b)]
+        y = models.layer_norm(*leaves)
+        with torch.no_grad():
+            leaves[i].add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward(dy.to(dev))
+    leaves = [t.to(dev).requires_grad_(True) for t in (x, w, b)]
+    y = checkpoint(models.layer_norm, *leaves, use_reentrant=False)
+    for name, g in zip(("dx", "dw", "db"), torch.autograd.grad(y, leaves, dy.to(dev))):
+        check(g, want[name], f"checkpointed {name}")
+
+
+def test_rms_norm_with_a_bias_and_modulation_in_other_shapes(dev):
+    from unirl_amd import models, ops
+
+    x, w, b, dy = make((19, 200), torch.float16, 22, False)
+    want = reference(x, w, b, dy, 1e-5, True, 0.0)
+    args = [t.to(dev) for t in (x, w, b)]
+    y, mean, rstd = ops.layer_norm(*args, rms=True, want_stats=True)
+    assert mean is None
+    check(y, want["y"], "y")
+    got = ops.layer_norm_bwd(dy.to(dev), args[0], None, rstd, *args[1:], rms=True)
+    for name, g in zip(("dx", "dw", "db"), got):
+        check(g, want[name], name)
+    # [B, D], [B, h, w, D], a permuted [B, D, h, w] and a gain broadcast over the samples
+    for shape in ((5, 72), (3, 2, 5, 72)):
+        x, w, b, dy = make(shape, torch.bfloat16, 23, True)
+        want = reference(x, w, b, dy, 1e-6, False, 1.0)
+        got = run(x, w, b, dy, 1e-6, "mod", dev)
+        for name in want:
+            check(got[name], want[name], f"{shape} {name}")
+    picture = x.permute(0, 3, 1, 2).contiguous().to(dev).permute(0, 2, 3, 1)
+    assert not picture.is_contiguous()
+    check(models.modulated_layer_norm(picture, w.to(dev), b.to(dev)), want["y"], "permuted")
+    one_w, one_b = w[:1].to(dev).requires_grad_(True), b[:1].to(dev).requires_grad_(True)
+    y = models.modulated_layer_norm(x.to(dev), one_w.expand(3, 72), one_b.expand(3, 72))
+    gw, gb = torch.autograd.grad(y, (one_w, one_b), dy.to(dev))
+    same = reference(x, w[:1].expand(3, 72), b[:1].expand(3, 72), dy, 1e-6, False, 1.0)
+    check(y, same["y"], "one modulation")
+    for g, name in ((gw, "dw"), (gb, "db")):  # the sum over samples is autograd's, in bf16: one rounding more per sample
+        value, bound = same[name]
+        check(g, (value.sum(0, keepdim=True), bound.sum(0, keepdim=True) + 3 * half(torch.bfloat16) * value.abs().sum(0, keepdim=True)),
+              name)
+
+
 def test_replay_log_prob_behind_a_final_norm(dev):
     """chunked_replay_logp(final_norm=...) on hidden states from before the norm: the same log-probs and
     gradients as the norm called in front of it, and the gain's gradient."""

@@ -355,7 +355,7 @@ def test_8_bit_averages_are_unbiased(dev):
 
 def test_dither_depends_on_seed_step_and_position_alone(dev):
     def go(**kw):
-        T, D = make([3000, 777], torch.float32, torch.float32, 8, False, 6, dev)
+        T, D = make([2000, 777], torch.float32, torch.float32, 8, False, 6, dev)
         apply(D, dict(HYPER, step=kw.pop("step", 3)), **kw)
         return [d["m"] for d in D], D
 
@@ -365,8 +365,8 @@ def test_dither_depends_on_seed_step_and_position_alone(dev):
     for kw in (dict(seed=2), dict(seed=1, step=4), dict(seed=1, index_bases=[256, 1 << 20])):
         assert not torch.equal(a[0], go(**kw)[0][0])
     # one tensor alone, with its own base, gives the same bytes as in the list; positions beyond 2^32 count
-    T, D = make([3000, 777], torch.float32, torch.float32, 8, False, 6, dev)
-    apply(D[1:], HYPER, seed=1, index_bases=[3072])
+    T, D = make([2000, 777], torch.float32, torch.float32, 8, False, 6, dev)
+    apply(D[1:], HYPER, seed=1, index_bases=[2048])
     assert torch.equal(D[1]["m"], a[1])
     far = go(seed=1, index_bases=[(1 << 33) + 256, 1 << 40])[1]
     for (t, d, base) in zip(T, far, [(1 << 33) + 256, 1 << 40]):
@@ -447,6 +447,75 @@ def test_device_counter_and_captured_steps(dev):
             compare()
             assert int(count) == taken
         lr.fill_(1e-3)
+
+
+def test_streams_and_graphs_do_not_share_scratch(dev):
+    """Norms of different gradients on two streams at once, and of two graphs replayed in turn with eager
+    calls between: each gives the value of its own input."""
+    from unirl_amd import ops
+
+    sets = [[torch.randn(3_000_001 + 7 * k + i, device=dev) * (k + 1) for i in range(5)] for k in range(2)]
+    want = [float(ops.grad_norm(s)) for s in sets]
+    assert want[0] != want[1]
+    streams = [torch.cuda.Stream(dev) for _ in sets]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[k].append(ops.grad_norm(sets[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(float(v) == want[k] for v in got[k])
+    graphs, outs = [], []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.grad_norm(s))
+        graphs.append(graph)
+    for _ in range(4):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                outs[k].zero_()
+                graphs[k].replay()
+        torch.cuda.synchronize()
+        assert [float(v) for v in outs] == want
+        assert float(ops.grad_norm(sets[0] + sets[1])) > max(want)
+
+
+def test_first_step_that_is_skipped(dev):
+    """A bad gradient in the first step: nothing is written, nothing counted; the next step is step 1."""
+    from unirl_amd.train import AdamW
+
+    for bits in (32, 8):
+        ours, twin = model(torch.bfloat16, dev), model(torch.bfloat16, dev)
+        kw = dict(lr=1e-2, state_bits=bits, master_weights=True)
+        a, b = AdamW(ours, capturable=True, skip_nonfinite=True, **kw), AdamW(twin, **kw)
+        set_grads(ours, 0)
+        ours[1].grad[3] = float("inf")
+        before = [p.detach().clone() for p in ours]
+        a.step()
+        assert math.isinf(float(a.grad_norm)) and int(a.param_groups[0]["step"]) == 0
+        assert all(torch.equal(p, q) for p, q in zip(ours, before))
+        for k in range(2):
+            set_grads(ours, k)
+            set_grads(twin, k)
+            a.step()
+            b.step()
+        assert all(torch.equal(p, q) for p, q in zip(ours, twin)) and int(a.param_groups[0]["step"]) == 2
+
+
+def test_a_step_between_forward_and_backward_is_noticed(dev):
+    from unirl_amd import models
+    from unirl_amd.train import AdamW
+
+    w = torch.nn.Parameter(torch.ones(64, device=dev))
+    x = torch.randn(5, 64, device=dev, requires_grad=True)
+    y = models.rms_norm(x, w)
+    w.grad = torch.ones_like(w)
+    AdamW([w]).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
 
 
 def test_refusals(dev):
