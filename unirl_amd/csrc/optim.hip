@@ -49,11 +49,13 @@ __device__ __forceinline__ int find_tensor(const uint32_t* first, uint32_t b) {
 
 // Sum of squares of [p, p + n) over the workgroup's threads, one value per thread.  The squares are
 // formed and added in fp64: exact for every fp32 product, no overflow or underflow for any finite
-// gradient.
+// gradient.  Bound by reading: 400 M bf16 elements in 117 us (6.8 TB/s).  Small lists are bound by the
+// launch (160 tensors of 5 M elements together 7 us); two loads a lane in flight suit both (one: 8.5, four:
+// 7.7, eight: 9.1 us for the small list, whose code is fetched anew by every launch).
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ double thread_sumsq(const T* p, int64_t n) {
   constexpr int VEC = ALIGNED ? 16 / (int)sizeof(T) : 1;
-  constexpr int U = 4;  // 16-byte loads in flight per lane
+  constexpr int U = 2;  // loads in flight per lane
   double a[2] = {0.0, 0.0};
   const int64_t step = (int64_t)kGradNormThreads * VEC;
   int64_t i = (int64_t)threadIdx.x * VEC;
@@ -421,8 +423,10 @@ __device__ __forceinline__ void adamw_blocks(const AdamCommon& A, const AdamCont
   }
 }
 
-// Bound by HBM: 28 bytes an element with 32-bit moments and a master, 10 with 8-bit moments and a
-// 16-bit parameter.  A lane takes four elements of a block, so that a block's maximum is one reduction
+// Bound by HBM: 28 bytes an element with 32-bit moments and a master, 16 with 8-bit moments and a master
+// (10 without).  400 M bf16 elements with masters: 2.05 ms and 1.15 ms, 5.5 and 5.6 TB/s, the rate of a copy
+// on this card; streaming accesses (temporal ones: 2.10 ms), workgroups in address order (a range of its
+// own for each XCD: the same).  A lane takes four elements of a block, so that a block's maximum is one reduction
 // inside a wavefront.
 template <typename P, typename G, int BITS, bool MASTER>
 __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs<BITS, MASTER> A) {
@@ -484,8 +488,9 @@ __global__ void adamw_advance_kernel(int64_t* step, AdamControl* control, AdamSc
 }
 
 // The values that 8-bit moments stand for: eight elements a lane (a lane's stores are 16 bytes in 16-bit
-// types), four times; blockIdx.y: m, v.
-constexpr int kMomentsChunk = 256 * 8 * 4;
+// types), kMomentsRounds times; blockIdx.y: m, v.  Bound by HBM: 400 M elements to bf16 in 394 us (6.1 TB/s).
+constexpr int kMomentsRounds = 2;
+constexpr int kMomentsChunk = 256 * 8 * kMomentsRounds;
 template <typename O>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t* m, const uint8_t* v, const uint8_t* sm,
                                                             const uint8_t* sv, int64_t n, O* out_m, O* out_v, int aligned) {
@@ -501,16 +506,16 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t* m, co
   };
   for (int64_t e0 = (int64_t)blockIdx.x * kMomentsChunk; e0 < n; e0 += (int64_t)gridDim.x * kMomentsChunk) {
     if (aligned && e0 + kMomentsChunk <= n) {
-      u32x2 w[4];
-      uint32_t s[4];
+      u32x2 w[kMomentsRounds];
+      uint32_t s[kMomentsRounds];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kMomentsRounds; ++u) {
         const int64_t i = e0 + u * 2048 + threadIdx.x * 8;
         w[u] = stream_load8(codes + i);
         s[u] = scales[i / kQuantBlock];
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kMomentsRounds; ++u) {
         float lo[4], hi[4], o[8];
         decode(w[u].x, scale_of(s[u]), lo);
         decode(w[u].y, scale_of(s[u]), hi);
@@ -519,7 +524,7 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t* m, co
         Vec<O, 8>::store(out + e0 + u * 2048 + threadIdx.x * 8, o);
       }
     } else {
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kMomentsRounds; ++u) {
         const int64_t i = e0 + u * 2048 + threadIdx.x * 8;
         if (i >= n) break;
         const float scale = scale_of(scales[i / kQuantBlock]);
