@@ -687,6 +687,24 @@ def test_master_weights_keep_small_updates(dev):
         assert bool((p == (1 + 2 * 2.0**-7 if master else 1.0)).all())
 
 
+def test_masters_follow_written_parameters_on_request(dev):
+    from unirl_amd.train import AdamW
+
+    p = torch.nn.Parameter(torch.ones(8, device=dev, dtype=torch.bfloat16))
+    opt = AdamW([p], lr=0.0, weight_decay=0.0, master_weights=True)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with torch.no_grad():
+        p.fill_(3.0)
+    opt.step()
+    assert bool((p == 1.0).all())  # the master leads
+    with torch.no_grad():
+        p.fill_(3.0)
+    opt.refresh_masters()
+    opt.step()
+    assert bool((p == 3.0).all())
+
+
 def test_captured_optimizer(dev):
     from unirl_amd.train import AdamW
 

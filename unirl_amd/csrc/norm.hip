@@ -620,7 +620,7 @@ static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool b
     if (S.threads <= 512) {
       if (backward)
         hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, BIAS, 512>), grid, block, kSlots, s, A);
-      else
+      else if constexpr (VEC == 1 || E > 8)  // vectors of so narrow rows belong to one wavefront
         hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, false, BIAS, 512>), grid, block, 0, s, A);
     } else if constexpr (E == 32) {
       if (backward)
@@ -791,11 +791,13 @@ extern "C" int unirl_layer_norm_bwd(const struct unirl_norm_desc* d, const void*
     if (dy_group_stride < 0 || dy_row_stride < 0) return UNIRL_E_SHAPE;
     if (!aligned_to(dy, es) || !aligned_to(dx, es)) return UNIRL_E_ALIGN;
     const bool vectors = vectors_ok(d->x, d->x_group_stride, d->x_row_stride, d->D, d->groups, d->rows, es) &&
-                         vectors_ok(dy, dy_group_stride, dy_row_stride, d->D, d->groups, d->rows, es) && params_vectors_ok(d) && aligned_to(dx, 16);
+                         vectors_ok(dy, dy_group_stride, dy_row_stride, d->D, d->groups, d->rows, es) &&
+                         params_vectors_ok(d) && aligned_to(dx, 16);
     const NormShape S = norm_shape(d->D, d->dtype, vectors, true);
     blocks = norm_blocks(S, d->groups, d->rows, true);
     if (params) {
-      if (!scratch || scratch_bytes < unirl_layer_norm_bwd_scratch_bytes(d->groups, d->rows, d->D)) return UNIRL_E_WORKSPACE;
+      if (!scratch || scratch_bytes < unirl_layer_norm_bwd_scratch_bytes(d->groups, d->rows, d->D))
+        return UNIRL_E_WORKSPACE;
       if (!aligned_to(scratch, 16)) return UNIRL_E_ALIGN;
       // the launch's own partial rows, whatever the function above says
       if ((size_t)(d->groups * blocks * d->D) * (dbias ? 2 : 1) * sizeof(float) > scratch_bytes) return UNIRL_E_WORKSPACE;

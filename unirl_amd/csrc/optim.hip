@@ -115,9 +115,10 @@ __global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* pa
 // ---------------------------------------------------------------------------
 constexpr int kAdamThreads = 256;
 constexpr int kQuantBlock = 256;  // elements that share a scale: one wavefront's four elements a lane
-// Blocks of one wavefront, whose loads are in flight together.  With 32-bit moments one block is
-// enough (eight wavefronts a SIMD keep the memory busy) and the shorter code is fetched sooner: a launch over 1.6 M elements takes 10.2 us with one block, 10.4 with two, 11.3 with four,
-// one over 400 M 2.02, 2.10, 2.06 ms.  With 8-bit moments: 9.3 / 9.6 / 11.3 us and 1.20 / 1.14 / 1.16 ms.
+// Blocks of one wavefront, whose loads are in flight together.  With 32-bit moments one block is enough
+// (eight wavefronts a SIMD keep the memory busy) and the shorter code is fetched sooner: a launch over 1.6 M
+// elements takes 10.2 us with one block, 10.4 with two, 11.3 with four, one over 400 M 2.02, 2.10, 2.06 ms.
+// With 8-bit moments: 9.3 / 9.6 / 11.3 us and 1.20 / 1.14 / 1.16 ms.
 constexpr int adam_unroll(int bits) { return bits == 32 ? 1 : 2; }
 constexpr int64_t kMaxGrid = 0xffffff;  // workgroups of 256 threads: a launch counts its threads in 32 bits
 constexpr int adam_chunk(int bits) { return kAdamThreads / kWave * adam_unroll(bits) * kQuantBlock; }
@@ -224,7 +225,6 @@ __device__ __forceinline__ uint32_t wave_pk_max_u16(uint32_t v) {
   UNIRL_DPP_REDUCE(v, pk_max_u16, dpp_u32_or_zero)
   return last_lane(v);
 }
-
 
 // One lane's four consecutive elements of one block, in registers.
 template <typename P, typename G, int BITS, bool MASTER>
@@ -426,8 +426,8 @@ __device__ __forceinline__ void adamw_blocks(const AdamCommon& A, const AdamCont
 // Bound by HBM: 28 bytes an element with 32-bit moments and a master, 16 with 8-bit moments and a master
 // (10 without).  400 M bf16 elements with masters: 2.05 ms and 1.15 ms, 5.5 and 5.6 TB/s, the rate of a copy
 // on this card; streaming accesses (temporal ones: 2.10 ms), workgroups in address order (a range of its
-// own for each XCD: the same).  A lane takes four elements of a block, so that a block's maximum is one reduction
-// inside a wavefront.
+// own for each XCD: the same).  A lane takes four elements of a block, so that a block's maximum is one
+// reduction inside a wavefront.
 template <typename P, typename G, int BITS, bool MASTER>
 __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs<BITS, MASTER> A) {
   AdamControl C = A.host;

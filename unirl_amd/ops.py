@@ -1632,8 +1632,8 @@ def adamw_step(
     with ``skip_nonfinite`` nothing is written when the norm is Inf or NaN.
 
     ``params`` share one dtype, ``grads`` the same one or fp32; all tensors are contiguous and must not
-    overlap.  ``masters`` (fp32) hold the values of 16-bit ``params``, which then receive the rounded
-    master.  The moments are fp32, or uint8 together with ``exp_avg_scales`` / ``exp_avg_sq_scales``
+    overlap.  ``masters`` (fp32) hold the values of 16-bit ``params``, which are then not read and receive
+    the rounded master.  The moments are fp32, or uint8 together with ``exp_avg_scales`` / ``exp_avg_sq_scales``
     (uint8, one per 256 elements; zeros are the zero state): formats and stochastic rounding as in
     :func:`adamw_moments`.  The rounding's random bits are a hash of ``(seed, step, index_bases[i] +
     element)``; ``index_bases`` (multiples of 256) default to the tensors laid end to end.

@@ -22,7 +22,8 @@ class AdamW(torch.optim.Optimizer):
     ``state_bits``: moments in fp32 (32), or in one byte each with a power-of-two scale per 256
     elements (8; formats in :func:`unirl_amd.ops.adamw_moments`).  ``master_weights`` keeps an fp32 copy of
     16-bit parameters, without which updates below half a unit in the last place of a parameter are
-    lost.  Both may be set per parameter group.
+    lost; it is made in a parameter's first step and leads from then on, so parameters written by
+    hand (loaded weights) need :meth:`refresh_masters`.  Both may be set per parameter group.
 
     ``max_grad_norm`` clips by the global norm of all groups' gradients; ``step()`` leaves that norm in
     ``grad_norm`` (a device scalar; ``None`` without ``max_grad_norm`` and ``skip_nonfinite``).
@@ -115,6 +116,13 @@ class AdamW(torch.optim.Optimizer):
         if "exp_avg_scale" not in s:
             return s["exp_avg"], s["exp_avg_sq"]
         return ops.adamw_moments(s["exp_avg"], s["exp_avg_sq"], s["exp_avg_scale"], s["exp_avg_sq_scale"])
+
+    @torch.no_grad()
+    def refresh_masters(self) -> None:
+        """Take the fp32 masters anew from the parameters as they are."""
+        for p, s in self.state.items():
+            if "master" in s:
+                s["master"].copy_(p)
 
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
         """State tensors keep the dtypes they were saved with (the base class casts them to the
