@@ -579,16 +579,18 @@ struct NormShape {
   int vec, elems, threads;
 };
 // Rows of up to 32 vectors share a wavefront (forward, bf16 [781250, 128]: 76 us, one row a wavefront 183).
-// Rows of up to 64 * 64 elements (forward) or 64 * 32 (backward, whose lanes hold five numbers per
-// element: 40 spill with a bias and gain nothing without, 27.5 and 27.1 us for bf16 [8192, 2560]) belong to one
-// wavefront, longer ones to a workgroup of as few elements a lane (8, 16, 32) as 512 threads allow,
-// since wider workgroups leave too few registers or too few of them resident (backward, bf16
-// [13950, 7168]: 896 threads of 8 elements 229 us, 448 of 16 116 us).  Behind 16384 elements 1024 threads
-// spill in the backward (0.7 to 1.4 TB/s), which such rows have to bear.
+// Rows of up to 64 * 64 elements (forward; 64 * 32 one by one) or 64 * 32 (backward, whose lanes hold five
+// numbers per element; 64 * 24 in fp32, 64 * 16 one by one, which hold their loads in more registers)
+// belong to one wavefront, longer ones to a workgroup of as few elements a lane (8, 16, 32) as 512
+// threads allow, since wider workgroups leave too few registers or too few of them resident.  Backward
+// with a bias, 100 M elements, one wavefront / workgroup: bf16 D = 1600 101 / 123 us, 2560 120 / 103 us; fp32
+// D = 1600 (half as many) 133 / 104 us; bf16 D = 1500 element by element 170 / 144 us.  bf16 D = 7168: 896 threads
+// of 8 elements 229 us, 448 of 16 107 us.  Behind 16384 elements 1024 threads spill in the backward (0.7 to
+// 1.4 TB/s), which such rows have to bear.
 static NormShape norm_shape(int64_t D, int dtype, bool vectors, bool backward) {
   NormShape S;
   S.vec = vectors ? 16 / (int)dtype_size(dtype) : 1;
-  const int64_t one_wave = vectors && !backward ? 64 : 32;
+  const int64_t one_wave = !backward ? (vectors ? 64 : 32) : (!vectors ? 16 : (dtype == UNIRL_F32 ? 24 : 32));
   if (vectors && D <= 32 * S.vec) {
     S.lanes = D <= 8 * S.vec ? 8 : (D <= 16 * S.vec ? 16 : 32);
     S.elems = S.vec;
@@ -634,7 +636,7 @@ static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool b
   if (S.lanes == kWave) {
     if (!backward)
       hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, true, BIAS, kNormFwdRows * kWave>), grid, block, 0, s, A);
-    else if constexpr (E <= 32)
+    else if constexpr (E <= (VEC == 1 ? 16 : (sizeof(T) == 4 ? 24 : 32)))
       hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, true, BIAS, kNormBwdRows * kWave>), grid, block,
                          (size_t)A.D * (kNormBwdRows / 2 * 4), s, A);
   } else if constexpr (E == 8 || E == 16 || E == 32) {
