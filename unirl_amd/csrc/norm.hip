@@ -34,7 +34,7 @@ struct NormArgs {
   int gain_dtype;
   float gain_offset;
   int center;
-  bool keep_x;  // forward: x is small enough to stay cached
+  bool keep;  // what is read stays cached
   float eps, inv_d;
   uint32_t D;
   int64_t rows;
@@ -51,15 +51,15 @@ struct NormArgs {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* row, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(row), 0, bytes, 0x00020000);
 }
-// Cache policy.  What is read next stays cached: y and dx (their consumer follows), and in the forward x
-// (the residual stream, and the backward, read it again), unless it is too large to stay.  The backward's
-// x and dy are streamed past the caches: nobody reads them after it.  Streaming y and dx as well took 71.6
-// instead of 62.2 us for a forward of 201 MB and 60.8 instead of 57.6 us for a backward of 3 x 101 MB;
-// keeping x in the forward takes 54.1 instead of 57.6 us off that backward when it follows at once, but
-// 76.4 instead of 62.2 us for the 201 MB forward, whose x pushes out its y.
+// Cache policy, measured with calls back to back on three sets of inputs (a kernel timed alone leaves the
+// write-back of its cached stores to the next one).  Stores stream: cached ones take 39.2 instead of 35.0 us
+// for a forward of 101 MB, 77.0 instead of 73.3 us for 201 MB.  The forward's x stays cached where it is
+// read again or small: cached / streaming 15.2 / 17.5 us at 42 MB, 35.0 / 35.9 at 101 MB, 73.3 / 71.1 at 201 MB,
+// but with the backward behind it 169 / 177 us there.  The backward's x and dy are cached where they are small:
+// forward + backward 46.3 / 49.3 us at 42 MB, 66.1 / 65.6 at 63 MB, 179 / 169 at 201 MB.
 constexpr int kStreaming = 2;
 constexpr int kCached = 0;
-constexpr int64_t kKeepBytes = 128 << 20;  // half of the last-level cache
+constexpr int64_t kKeepForward = 128 << 20, kKeepBackward = 48 << 20;  // bytes of x
 
 // VEC consecutive elements of T as loaded (up to 16 bytes), and as floats.
 template <typename T, int VEC>
@@ -101,11 +101,11 @@ template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(__amdgpu_buffer_rsrc_t r, uint32_t off, const float (&o)[VEC]) {
   if constexpr (VEC == 1) {
     if constexpr (sizeof(T) == 4) {
-      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[0]), r, off, 0, kCached);
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[0]), r, off, 0, kStreaming);
     } else {
       T t;
       Elem<T>::store(&t, o[0]);
-      __builtin_amdgcn_raw_buffer_store_b16((short)t.bits, r, off, 0, kCached);
+      __builtin_amdgcn_raw_buffer_store_b16((short)t.bits, r, off, 0, kStreaming);
     }
   } else {
     u32x4 v;
@@ -118,7 +118,7 @@ __device__ __forceinline__ void store_vec(__amdgpu_buffer_rsrc_t r, uint32_t off
       else
         v[k] = f32_to_f16_bits(o[2 * k]) | (f32_to_f16_bits(o[2 * k + 1]) << 16);
     }
-    __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, kCached);
+    __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, kStreaming);
   }
 }
 
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormArgs A) {
   const int64_t group = blockIdx.y;
   const T* x = (const T*)A.x + group * A.x_group_stride;
   RowRegs<T, VEC, E> raw;
-  raw.load(x + first * A.x_row_stride, A.D, col, step, A.keep_x);
+  raw.load(x + first * A.x_row_stride, A.D, col, step, A.keep);
   float w[E], b[BIAS ? E : 1];
   load_param<VEC, E>(A.gain, A.gain_dtype, group * A.gain_group_stride, A.D, col, step, 1.0f, A.gain_offset, w);
   if constexpr (BIAS) load_param<VEC, E>(A.bias, A.gain_dtype, group * A.bias_group_stride, A.D, col, step, 0.0f, 0.0f, b);
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormArgs A) {
   for (int64_t row = first; row < A.rows; row += stride) {
     float v[E];
     raw.unpack(v);
-    if (row + stride < A.rows) raw.load(x + (row + stride) * A.x_row_stride, A.D, col, step, A.keep_x);
+    if (row + stride < A.rows) raw.load(x + (row + stride) * A.x_row_stride, A.D, col, step, A.keep);
     float mean = 0.0f;
     if (A.center) {
       float s = 0.0f;
@@ -260,8 +260,8 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormArgs A) {
   RowRegs<T, VEC, E> rx, rg;
   float rstd = 0.0f, mean = 0.0f;
   if (first < A.rows) {
-    rx.template load<kStreaming>(x + first * A.x_row_stride, A.D, col, step);
-    rg.template load<kStreaming>(dy + first * A.dy_row_stride, A.D, col, step);
+    rx.load(x + first * A.x_row_stride, A.D, col, step, A.keep);
+    rg.load(dy + first * A.dy_row_stride, A.D, col, step, A.keep);
   }
   float w[E];
   load_param<VEC, E>(A.gain, A.gain_dtype, group * A.gain_group_stride, A.D, col, step, 1.0f, A.gain_offset, w);
@@ -280,8 +280,8 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormArgs A) {
     rx.unpack(xh);
     rg.unpack(g);
     if (row + stride < A.rows) {
-      rx.template load<kStreaming>(x + (row + stride) * A.x_row_stride, A.D, col, step);
-      rg.template load<kStreaming>(dy + (row + stride) * A.dy_row_stride, A.D, col, step);
+      rx.load(x + (row + stride) * A.x_row_stride, A.D, col, step, A.keep);
+      rg.load(dy + (row + stride) * A.dy_row_stride, A.D, col, step, A.keep);
     }
     // behind the row's end x and dy are 0, and so is xh there (0 - mean could overflow on its way)
 #pragma unroll
@@ -429,7 +429,7 @@ __global__ __launch_bounds__(256) void norm_narrow_fwd_kernel(NormArgs A) {
   if (row >= A.rows) return;
   Packed<T, VEC> raw;
   const auto load = [&](int64_t r) {
-    if (A.keep_x)
+    if (A.keep)
       raw.template load<kCached>(at.rsrc(x, r, A.x_row_stride), at.off(r, A.rows, A.x_row_stride));
     else
       raw.template load<kStreaming>(at.rsrc(x, r, A.x_row_stride), at.off(r, A.rows, A.x_row_stride));
@@ -485,8 +485,13 @@ __global__ __launch_bounds__(512) void norm_narrow_bwd_kernel(NormArgs A) {
   Packed<T, VEC> rx, rg;
   float rstd = 0.0f, mean = 0.0f;
   const auto load = [&](int64_t r) {
-    rx.template load<kStreaming>(at.rsrc(x, r, A.x_row_stride), at.off(r, A.rows, A.x_row_stride));
-    rg.template load<kStreaming>(at.rsrc(dy, r, A.dy_row_stride), at.off(r, A.rows, A.dy_row_stride));
+    if (A.keep) {
+      rx.template load<kCached>(at.rsrc(x, r, A.x_row_stride), at.off(r, A.rows, A.x_row_stride));
+      rg.template load<kCached>(at.rsrc(dy, r, A.dy_row_stride), at.off(r, A.rows, A.dy_row_stride));
+    } else {
+      rx.template load<kStreaming>(at.rsrc(x, r, A.x_row_stride), at.off(r, A.rows, A.x_row_stride));
+      rg.template load<kStreaming>(at.rsrc(dy, r, A.dy_row_stride), at.off(r, A.rows, A.dy_row_stride));
+    }
     const int64_t flat = group * A.rows + (r + at.sub < A.rows ? r + at.sub : A.rows - 1);
     rstd = A.rstd[flat];
     if (A.center) mean = A.mean[flat];
@@ -752,7 +757,6 @@ static NormArgs norm_args(const struct unirl_norm_desc* d, int64_t group0) {
   A.gain_dtype = d->gain_dtype;
   A.gain_offset = d->gain_offset;
   A.center = d->center;
-  A.keep_x = d->groups * d->rows * d->D * (int64_t)es <= kKeepBytes;
   A.eps = (float)d->eps;
   A.inv_d = 1.0f / (float)d->D;
   A.D = (uint32_t)d->D;
@@ -779,6 +783,7 @@ extern "C" int unirl_layer_norm_fwd(const struct unirl_norm_desc* d, void* y, vo
   for (int64_t g0 = 0; g0 < d->groups; g0 += kNormMaxGroups) {
     const int64_t ng = d->groups - g0 < kNormMaxGroups ? d->groups - g0 : kNormMaxGroups;
     NormArgs A = norm_args(d, g0);
+    A.keep = d->rstd || d->groups * d->rows * d->D * (int64_t)es <= kKeepForward;
     A.out = (char*)y + g0 * d->rows * d->D * (int64_t)es;
     const int64_t gx = norm_blocks(S, d->groups, d->rows, false);
     launch_norm(A, S, d->dtype, dim3((unsigned)gx, (unsigned)ng), false, d->bias != nullptr, (hipStream_t)stream);
@@ -832,6 +837,7 @@ extern "C" int unirl_layer_norm_bwd(const struct unirl_norm_desc* d, const void*
     for (int64_t g0 = 0; g0 < d->groups; g0 += kNormMaxGroups) {
       const int64_t ng = d->groups - g0 < kNormMaxGroups ? d->groups - g0 : kNormMaxGroups;
       NormArgs A = norm_args(d, g0);
+      A.keep = d->groups * d->rows * d->D * (int64_t)es <= kKeepBackward;
       A.dy = offset_ptr(dy, g0 * dy_group_stride, es);
       A.dy_group_stride = dy_group_stride;
       A.dy_row_stride = dy_row_stride;
