@@ -136,6 +136,18 @@ def test_longest_rows(dev, kind, D):
             check(got[name], want[name], f"{kind} {D} {dtype} {name}")
 
 
+@pytest.mark.parametrize("kind", ["layer", "rms", "mod"])
+@pytest.mark.parametrize("D", [10240, 10241, 12296, 16383, 16385, 24576, 24579, 32760, 32767])
+def test_long_rows_several_a_workgroup(dev, D, kind):
+    """More rows than workgroups of one row each stay resident: every one takes two or three in turn."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w, b, dy = make((2, 300, D) if kind == "mod" else (520, D), dtype, D, kind == "mod", bias=kind != "rms")
+        want = reference(x, w, b, dy, 1e-5, kind == "rms", 1.0 if kind == "mod" else 0.0)
+        got = run(x, w, b, dy, 1e-5, kind, dev)
+        for name in want:
+            check(got[name], want[name], f"{kind} {D} {dtype} {name}")
+
+
 def test_longer_rows_are_refused(dev):
     from unirl_amd import models
 

@@ -201,9 +201,16 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormArgs A) {
   const T* x = (const T*)A.x + group * A.x_group_stride;
   RowRegs<T, VEC, E> raw;
   raw.load(x + first * A.x_row_stride, A.D, col, step, A.keep);
-  float w[E], b[BIAS ? E : 1];
-  load_param<VEC, E>(A.gain, A.gain_dtype, group * A.gain_group_stride, A.D, col, step, 1.0f, A.gain_offset, w);
-  if constexpr (BIAS) load_param<VEC, E>(A.bias, A.gain_dtype, group * A.bias_group_stride, A.D, col, step, 0.0f, 0.0f, b);
+  // 128 registers a lane hold a row and the next, but the gain and bias only behind packed loads: fp32
+  // D = 18432 77 us with them read per row, 96 us held; bf16 82 / 72 us
+  constexpr bool kHeld = THREADS < 1024 || (VEC > 1 && sizeof(T) == 2);
+  constexpr int kParams = kHeld ? E : 8;
+  float w[kParams], b[BIAS ? kParams : 1];
+  const auto load_params = [&](uint32_t at) {
+    load_param<VEC, kParams>(A.gain, A.gain_dtype, group * A.gain_group_stride, A.D, at, step, 1.0f, A.gain_offset, w);
+    if constexpr (BIAS) load_param<VEC, kParams>(A.bias, A.gain_dtype, group * A.bias_group_stride, A.D, at, step, 0.0f, 0.0f, b);
+  };
+  if constexpr (kHeld) load_params(col);
 
   for (int64_t row = first; row < A.rows; row += stride) {
     float v[E];
@@ -228,11 +235,14 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormArgs A) {
     const __amdgpu_buffer_rsrc_t y = row_rsrc((T*)A.out + flat * A.D, A.D * (uint32_t)sizeof(T));
 #pragma unroll
     for (int j = 0; j < E / VEC; ++j) {
+      if constexpr (!kHeld)
+        if (j % (8 / VEC) == 0) load_params(col + j * step);
       float o[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         const float xh = v[j * VEC + k] * rstd;
-        o[k] = BIAS ? fmaf(xh, w[j * VEC + k], b[BIAS ? j * VEC + k : 0]) : xh * w[j * VEC + k];
+        const int at = kHeld ? j * VEC + k : (j * VEC + k) % 8;
+        o[k] = BIAS ? fmaf(xh, w[at], b[BIAS ? at : 0]) : xh * w[at];
       }
       store_vec<T, VEC>(y, (col + j * step) * (uint32_t)sizeof(T), o);
     }
@@ -244,10 +254,15 @@ __global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormArgs A) {
 }
 
 // The sums of the columns stay in registers as well; a workgroup leaves one partial row per sum, and
-// norm_param_kernel adds those in order.
+// norm_param_kernel adds those in order.  Sixteen wavefronts a compute unit have 128 registers each:
+// there dgain's sums lie in LDS, and rows of more than 16384 elements are loaded when they are due and
+// read the gain from the caches (bf16 with a bias, 100 M elements, D = 24576: 138 us, all of it in registers and
+// scratch memory 462; D = 32768 195 / 763 us; one by one D = 16385 254 / 574 us, 32767 425).
 template <typename T, int VEC, int E, bool ONE_WAVE, bool BIAS, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormArgs A) {
+  constexpr bool kSumsInLds = THREADS == 1024, kAhead = THREADS < 1024 || E < 24, kGainHeld = kAhead;
   extern __shared__ float sums[];  // ONE_WAVE: 4 D floats to join the wavefronts; else 2 x 2 x 16 floats
+  __shared__ float dw_lds[kSumsInLds ? E * THREADS : 1];
   const uint32_t tid = ONE_WAVE ? threadIdx.x & (kWave - 1) : threadIdx.x;
   const uint32_t step = (ONE_WAVE ? kWave : blockDim.x) * VEC;
   const uint32_t col = tid * VEC;
@@ -259,15 +274,21 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormArgs A) {
   const int64_t stride = ONE_WAVE ? (int64_t)gridDim.x * kNormBwdRows : (int64_t)gridDim.x;
   RowRegs<T, VEC, E> rx, rg;
   float rstd = 0.0f, mean = 0.0f;
-  if (first < A.rows) {
+  if (kAhead && first < A.rows) {
     rx.load(x + first * A.x_row_stride, A.D, col, step, A.keep);
     rg.load(dy + first * A.dy_row_stride, A.D, col, step, A.keep);
   }
-  float w[E];
-  load_param<VEC, E>(A.gain, A.gain_dtype, group * A.gain_group_stride, A.D, col, step, 1.0f, A.gain_offset, w);
-  float dw[E], db[BIAS ? E : 1];
+  const int64_t gain_at = group * A.gain_group_stride;
+  float w[kGainHeld ? E : 8];
+  if constexpr (kGainHeld) load_param<VEC, E>(A.gain, A.gain_dtype, gain_at, A.D, col, step, 1.0f, A.gain_offset, w);
+  float dw[kSumsInLds ? 1 : E], db[BIAS ? E : 1];
 #pragma unroll
-  for (int k = 0; k < E; ++k) dw[k] = 0.0f;
+  for (int k = 0; k < E; ++k) {
+    if constexpr (kSumsInLds)
+      dw_lds[k * THREADS + threadIdx.x] = 0.0f;
+    else
+      dw[k] = 0.0f;
+  }
 #pragma unroll
   for (int k = 0; k < (BIAS ? E : 1); ++k) db[k] = 0.0f;
 
@@ -276,10 +297,14 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormArgs A) {
     const int64_t flat = group * A.rows + row;
     rstd = A.rstd[flat];
     if (A.center) mean = A.mean[flat];
+    if constexpr (!kAhead) {
+      rx.template load<kStreaming>(x + row * A.x_row_stride, A.D, col, step);
+      rg.template load<kStreaming>(dy + row * A.dy_row_stride, A.D, col, step);
+    }
     float xh[E], g[E];
     rx.unpack(xh);
     rg.unpack(g);
-    if (row + stride < A.rows) {
+    if (kAhead && row + stride < A.rows) {
       rx.load(x + (row + stride) * A.x_row_stride, A.D, col, step, A.keep);
       rg.load(dy + (row + stride) * A.dy_row_stride, A.D, col, step, A.keep);
     }
@@ -293,9 +318,17 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormArgs A) {
     float c1 = 0.0f, c2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-      dw[k] = fmaf(g[k], xh[k], dw[k]);
+      if constexpr (!kGainHeld)
+        if (k % 8 == 0)
+          load_param<VEC, 8>(A.gain, A.gain_dtype, gain_at, A.D, col + k / VEC * step, step, 1.0f, A.gain_offset, w);
+      if constexpr (kSumsInLds) {
+        float& sum = dw_lds[k * THREADS + threadIdx.x];
+        sum = fmaf(g[k], xh[k], sum);
+      } else {
+        dw[k] = fmaf(g[k], xh[k], dw[k]);
+      }
       if constexpr (BIAS) db[k] += g[k];
-      g[k] *= w[k];
+      g[k] *= w[kGainHeld ? k : k % 8];
       c1 = fmaf(g[k], xh[k], c1);
       c2 += g[k];
     }
@@ -341,7 +374,8 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(NormArgs A) {
     float* out = A.partial + (which ? A.partial_bias : 0) + (group * gridDim.x + blockIdx.x) * A.D;
     float acc[E];
 #pragma unroll
-    for (int k = 0; k < E; ++k) acc[k] = which ? db[BIAS ? k : 0] : dw[k];
+    for (int k = 0; k < E; ++k)
+      acc[k] = which ? db[BIAS ? k : 0] : (kSumsInLds ? dw_lds[k * THREADS + threadIdx.x] : dw[kSumsInLds ? 0 : k]);
     if constexpr (ONE_WAVE) {
       // the second half of the wavefronts leaves its sums in LDS, the first adds its own, then every
       // thread adds the four sums of its columns
@@ -583,15 +617,17 @@ struct NormShape {
   int lanes;  // of one row: 8, 16, 32 or 64 of a wavefront, 0 = a workgroup
   int vec, elems, threads;
 };
-// Rows of up to 32 vectors share a wavefront (forward, bf16 [781250, 128]: 76 us, one row a wavefront 183).
+// Rows of up to 32 vectors share a wavefront (forward, bf16 [781250, 128]: 77 us, one row a wavefront 183).
 // Rows of up to 64 * 64 elements (forward; 64 * 32 one by one) or 64 * 32 (backward, whose lanes hold five
 // numbers per element; 64 * 24 in fp32, 64 * 16 one by one, which hold their loads in more registers)
-// belong to one wavefront, longer ones to a workgroup of as few elements a lane (8, 16, 32) as 512
-// threads allow, since wider workgroups leave too few registers or too few of them resident.  Backward
-// with a bias, 100 M elements, one wavefront / workgroup: bf16 D = 1600 101 / 123 us, 2560 120 / 103 us; fp32
-// D = 1600 (half as many) 133 / 104 us; bf16 D = 1500 element by element 170 / 144 us.  bf16 D = 7168: 896 threads
-// of 8 elements 229 us, 448 of 16 107 us.  Behind 16384 elements 1024 threads spill in the backward (0.7 to
-// 1.4 TB/s), which such rows have to bear.
+// belong to one wavefront, longer ones to a workgroup.  Backward with a bias, 100 M elements of bf16 (half
+// as many of fp32), one wavefront / workgroup: bf16 D = 1000 114 / 168 us, 1600 105 / 127 us, 2048 109 / 112 us;
+// fp32 equal from D = 1000 to 1536.
+// A workgroup has as few elements a lane as its width allows, since wide workgroups stay resident alone
+// and few registers hold a long row: backward 8 up to 768 threads (bf16 D = 5120 109 us, 16 of 320 threads
+// 134; but D = 7168 115 us in 16, 150 in 8 of 896 threads), then 16 (bf16 / fp32 D = 10240 135 / 113 us, 32 of 320
+// threads, some of them in scratch memory, 160 / 205), 24, 32.  Forward 8 and 16 up to 512 threads, then 32, and
+// 24 where that fits 1024 threads.
 static NormShape norm_shape(int64_t D, int dtype, bool vectors, bool backward) {
   NormShape S;
   S.vec = vectors ? 16 / (int)dtype_size(dtype) : 1;
@@ -608,7 +644,7 @@ static NormShape norm_shape(int64_t D, int dtype, bool vectors, bool backward) {
     S.threads = kWave * (backward ? kNormBwdRows : kNormFwdRows);
   } else {
     S.lanes = 0;
-    S.elems = D <= 512 * 8 ? 8 : (D <= 512 * 16 ? 16 : 32);
+    S.elems = D <= (backward ? 768 : 512) * 8 ? 8 : (D <= (backward ? 1024 : 512) * 16 ? 16 : (D > 512 * 32 && D <= 1024 * 24 ? 24 : 32));
     S.threads = (int)((D + S.elems * kWave - 1) / (S.elems * kWave)) * kWave;
   }
   return S;
@@ -644,18 +680,26 @@ static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool b
     else if constexpr (E <= (VEC == 1 ? 16 : (sizeof(T) == 4 ? 24 : 32)))
       hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, true, BIAS, kNormBwdRows * kWave>), grid, block,
                          (size_t)A.D * (kNormBwdRows / 2 * 4), s, A);
-  } else if constexpr (E == 8 || E == 16 || E == 32) {
+  } else if constexpr (E == 8 || E == 16 || E == 24 || E == 32) {
+    // what norm_shape gives: forward 8, 16, 32 up to 512 threads, 24, 32 above; backward 8 up to 768
+    // threads, 16 at any width, 24, 32 above 512
     constexpr size_t kSlots = 64 * 4;
-    if (S.threads <= 512) {
-      if (backward)
-        hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, BIAS, 512>), grid, block, kSlots, s, A);
-      else if constexpr (VEC == 1 || E > 8)  // vectors of so narrow rows belong to one wavefront
-        hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, false, BIAS, 512>), grid, block, 0, s, A);
-    } else if constexpr (E == 32) {
-      if (backward)
-        hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, BIAS, 1024>), grid, block, kSlots, s, A);
-      else
-        hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, false, BIAS, 1024>), grid, block, 0, s, A);
+    const bool small = S.threads <= 512;
+    if (backward) {
+      if constexpr (E <= 16)
+        if (small) hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, BIAS, 512>), grid, block, kSlots, s, A);
+      if constexpr (E <= 16)
+        if (!small && S.threads <= 768)
+          hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, BIAS, 768>), grid, block, kSlots, s, A);
+      if constexpr (E >= 16)
+        if (S.threads > (E == 16 ? 768 : 512))
+          hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, E, false, BIAS, 1024>), grid, block, kSlots, s, A);
+    } else {
+      // vectors of rows that 8 a lane cover belong to one wavefront
+      if constexpr (E != 24 && (VEC == 1 || E > 8))
+        if (small) hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, false, BIAS, 512>), grid, block, 0, s, A);
+      if constexpr (E >= 24)
+        if (!small) hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, E, false, BIAS, 1024>), grid, block, 0, s, A);
     }
   }
 }
@@ -691,6 +735,7 @@ static void launch_norm(const NormArgs& A, const NormShape& S, dim3 grid, bool b
     switch (S.elems) {
       case 8: return launch_norm<T, 1, 8>(A, S, grid, backward, bias, s);
       case 16: return launch_norm<T, 1, 16>(A, S, grid, backward, bias, s);
+      case 24: return launch_norm<T, 1, 24>(A, S, grid, backward, bias, s);
       default: return launch_norm<T, 1, 32>(A, S, grid, backward, bias, s);
     }
   }
