@@ -652,7 +652,7 @@ static NormShape norm_shape(int64_t D, int dtype, bool vectors, bool backward) {
 // Workgroups of one group.  Forward: up to 4 a compute unit (8 where rows share a wavefront).
 // Backward: as many as stay resident, since a few more would run alone behind the others, with two rows
 // a wavefront at least, since each leaves a partial row of D sums.
-static int64_t norm_blocks(const NormShape& S, int64_t groups, int64_t rows, bool backward) {
+static int64_t norm_blocks(const NormShape& S, int64_t groups, int64_t rows, bool backward, bool bias) {
   const int64_t rows_at_once = S.lanes ? S.threads / S.lanes : 1;
   const int64_t most = (rows + rows_at_once - 1) / rows_at_once;
   int64_t total = S.lanes && S.lanes < kWave ? 2 * kNormMaxBlocks : kNormMaxBlocks;
@@ -661,7 +661,11 @@ static int64_t norm_blocks(const NormShape& S, int64_t groups, int64_t rows, boo
     int64_t slots = S.elems <= 8 ? 28 : (S.elems <= 16 ? 16 : 8);
     if (S.vec == 1) slots = S.elems <= 8 ? 20 : (S.elems <= 16 ? 12 : 8);
     if (S.lanes && S.lanes < kWave) slots = 16;
-    const int64_t resident = slots / (S.threads / kWave);
+    const int64_t waves = S.threads / kWave;
+    // fewer where they do not spread evenly over its four register files, which a bias fills further (with it,
+    // 28 / these, bf16 D = 3584 140 / 113 us, 4608 134 / 109; fp32 D = 3584 120 / 111 us)
+    if (S.elems <= 8 && waves % 4) slots = S.vec == 8 ? (bias ? 24 : 28) : (S.vec == 4 ? (bias ? 22 : 24) : (bias ? 16 : 20));
+    const int64_t resident = slots / waves;
     total = 256 * (resident > 1 ? resident : 1);
     if (total > kNormMaxBlocks) total = kNormMaxBlocks;  // what unirl_layer_norm_bwd_scratch_bytes has room for
     const int64_t enough = (rows * groups + 2 * rows_at_once - 1) / (2 * rows_at_once);
@@ -830,7 +834,7 @@ extern "C" int unirl_layer_norm_fwd(const struct unirl_norm_desc* d, void* y, vo
     NormArgs A = norm_args(d, g0);
     A.keep = d->rstd || d->groups * d->rows * d->D * (int64_t)es <= kKeepForward;
     A.out = (char*)y + g0 * d->rows * d->D * (int64_t)es;
-    const int64_t gx = norm_blocks(S, d->groups, d->rows, false);
+    const int64_t gx = norm_blocks(S, d->groups, d->rows, false, false);
     launch_norm(A, S, d->dtype, dim3((unsigned)gx, (unsigned)ng), false, d->bias != nullptr, (hipStream_t)stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
@@ -869,7 +873,7 @@ extern "C" int unirl_layer_norm_bwd(const struct unirl_norm_desc* d, const void*
                          vectors_ok(dy, dy_group_stride, dy_row_stride, d->D, d->groups, d->rows, es) &&
                          params_vectors_ok(d) && aligned_to(dx, 16);
     const NormShape S = norm_shape(d->D, d->dtype, vectors, true);
-    blocks = norm_blocks(S, d->groups, d->rows, true);
+    blocks = norm_blocks(S, d->groups, d->rows, true, dbias != nullptr);
     if (params) {
       if (!scratch || scratch_bytes < unirl_layer_norm_bwd_scratch_bytes(d->groups, d->rows, d->D))
         return UNIRL_E_WORKSPACE;
