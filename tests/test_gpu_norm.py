@@ -366,6 +366,41 @@ def test_captured_forward_and_backward(dev):
                 assert torch.equal(o, e)
 
 
+def test_captured_autograd_and_a_living_eager_graph(dev):
+    """A captured backward is refused while a graph of the default stream over the same leaf is alive;
+    without one it is captured, and every replay gives the eager gradients."""
+    from unirl_amd import models
+
+    x = torch.randn(300, 520, device=dev).bfloat16()
+    dy = torch.randn_like(x)
+    w = torch.rand(520, device=dev).bfloat16().requires_grad_(True)
+
+    alive = models.rms_norm(x, w)
+    refused = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(refused):
+        y = models.rms_norm(x, w)
+        with pytest.raises(RuntimeError, match="alive"):
+            y.backward(dy)
+    assert w.grad is None
+    del alive, y, refused
+
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        models.rms_norm(x, w).backward(dy)
+    held = w.grad
+    for seed in range(3):
+        g = torch.Generator().manual_seed(seed)
+        x.copy_(torch.randn(x.shape, generator=g))
+        dy.copy_(torch.randn(x.shape, generator=g))
+        held.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.autograd.grad(models.rms_norm(x, w), w, dy)[0]
+        assert torch.equal(held, want)
+
+
 @pytest.mark.parametrize("bias", [False, True])
 def test_backward_stays_inside_its_scratch(dev, bias):
     """Scratch of exactly the documented size: the bytes behind it keep their values (and the entry point

@@ -14,6 +14,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/engine.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -273,6 +275,26 @@ void check(int rc, const char* what) {
   TORCH_CHECK_VALUE(rc >= 0, what, ": ", unirl_status_string(rc), " (status ", rc, ")");
   TORCH_CHECK(rc == 0, what, ": HIP error ", rc, ": ", unirl_status_string(rc));
 }
+// A leaf's accumulator works on the stream that was current when the first graph that still lives was
+// built over the leaf.  Where that is the default stream, the engine would make it wait for work that is
+// being captured, which breaks the capture and can end the process: refused while nothing is lost.
+void refuse_accumulators_outside_a_capture(int8_t device) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device).stream(), &status) != hipSuccess ||
+      status == hipStreamCaptureStatusNone)
+    return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const auto outside = c10::hip::getDefaultHIPStream(device);
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& to = node->next_edge(i).function;
+    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(to.get()) || !node->task_should_compute_output(i)) continue;
+    const auto stream = to->stream();
+    TORCH_CHECK(!stream || stream->id() != outside.id() || stream->device_index() != device,
+                "the norm's backward is captured while a graph built on the default stream over the same leaf is alive: "
+                "release that graph (its outputs and losses) before the captured forward");
+  }
+}
 using torch::autograd::variable_list;
 struct NormFunction : torch::autograd::Function<NormFunction> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight,
@@ -289,6 +311,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &mean = saved[3];
     const auto optional = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    refuse_accumulators_outside_a_capture(x.device().index());
     const size_t bias_edge = weight.defined() ? 2 : 1;  // only the tensors that are there have an edge
     NormGrads o;
     {
