@@ -1,0 +1,129 @@
+"""CPU-only checks of what ``train.AdamW`` does with saved states: what fits is taken over whole, what does
+not is refused before anything of the optimizer is replaced.  Nothing here takes a step."""
+
+import copy
+
+import pytest
+import torch
+
+SIZES = [(6, 50), (7,)]
+
+
+@pytest.fixture(scope="module")
+def AdamW(built_lib):
+    from unirl_amd.train import AdamW
+
+    return AdamW
+
+
+def params(dtype=torch.float32, device="cpu"):
+    return [torch.nn.Parameter(torch.zeros(s, dtype=dtype, device=device)) for s in SIZES]
+
+
+def saved_state(opt, steps, bits=32, master=False):
+    """A state as ``opt`` would have it after ``steps`` (one number per parameter, None: never a gradient)."""
+    sd = copy.deepcopy(opt.state_dict())
+    base = 0
+    for i, (p, n) in enumerate(zip([p for g in opt.param_groups for p in g["params"]], steps)):
+        blocks = -(-p.numel() // 256)
+        if n is not None:
+            dtype = torch.float32 if bits == 32 else torch.uint8
+            s = {"step": n, "index_base": base}
+            for name in ("exp_avg", "exp_avg_sq"):
+                s[name] = torch.arange(p.numel()).view(p.shape).to(dtype)
+                if bits == 8:
+                    s[name + "_scale"] = torch.full((blocks,), 100, dtype=torch.uint8)
+            if master:
+                s["master"] = torch.full(p.shape, 0.5)
+            sd["state"][i] = s
+        base += 256 * blocks
+    return sd
+
+
+def same(a, b):
+    if isinstance(a, dict):
+        return isinstance(b, dict) and a.keys() == b.keys() and all(same(a[k], b[k]) for k in a)
+    if isinstance(a, (list, tuple)):
+        return len(a) == len(b) and all(same(x, y) for x, y in zip(a, b))
+    if isinstance(a, torch.Tensor):
+        return isinstance(b, torch.Tensor) and a.dtype == b.dtype and torch.equal(a, b)
+    return a == b
+
+
+def test_a_fitting_state_is_taken_over_whole(AdamW):
+    for bits in (32, 8):
+        opt = AdamW(params(torch.bfloat16), state_bits=bits, master_weights=True)
+        sd = saved_state(opt, [4, None], bits, master=True)
+        sd["param_groups"][0]["lr"] = 0.25
+        opt.load_state_dict(sd)
+        assert same(opt.state_dict(), sd)
+        assert all(t.dtype == sd["state"][0][k].dtype and t is not sd["state"][0][k]
+                   for k, t in opt.state[opt.param_groups[0]["params"][0]].items() if isinstance(t, torch.Tensor))
+        assert opt._next_base == 512
+
+
+def test_hooks_see_and_change_what_is_loaded(AdamW):
+    opt = AdamW(params())
+    called = []
+
+    def before(o, sd):
+        sd = copy.deepcopy(sd)
+        sd["state"][0]["step"] = 9
+        return sd
+
+    opt.register_load_state_dict_pre_hook(before)
+    opt.register_load_state_dict_post_hook(lambda o: called.append(dict(o.state[o.param_groups[0]["params"][0]])))
+    opt.load_state_dict(saved_state(opt, [4, 4]))
+    assert called[0]["step"] == 9 and opt.state[opt.param_groups[0]["params"][0]]["step"] == 9
+
+
+def refused(sd):
+    """Variants of ``sd`` that do not fit, by name."""
+    def change(f):
+        c = copy.deepcopy(sd)
+        f(c)
+        return c
+
+    def pop(key):
+        return lambda c: c["state"][1].pop(key)
+
+    def put(key, value):
+        return lambda c: c["state"][1].update({key: value})
+
+    return {
+        "no index_base": change(pop("index_base")), "no step": change(pop("step")), "no second moment": change(pop("exp_avg_sq")),
+        "another shape": change(put("exp_avg_sq", torch.zeros(8))), "another dtype": change(put("exp_avg", torch.zeros(7).bfloat16())),
+        "not a tensor": change(put("exp_avg", 0.0)), "unaligned base": change(put("index_base", 100)),
+        "a master of another shape": change(put("master", torch.zeros(8))),
+        "a group less": change(lambda c: c["param_groups"].pop()),
+        "a parameter less": change(lambda c: c["param_groups"][0]["params"].pop()),
+        "no seed": change(lambda c: c["param_groups"][0].pop("seed")),
+        "betas out of range": change(lambda c: c["param_groups"][0].update(betas=(1.0, 0.9))),
+    }
+
+
+def test_a_refused_state_leaves_the_optimizer_as_it_was(AdamW):
+    ps = params()
+    opt = AdamW(ps, lr=1e-2)
+    opt.load_state_dict(saved_state(opt, [3, 3]))
+    before = copy.deepcopy(opt.state_dict())
+    sd = saved_state(opt, [5, 5])
+    sd["param_groups"][0]["lr"] = 1.0
+    plain = torch.optim.AdamW(params())
+    for p in plain.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    plain.step()
+    for name, bad in {**refused(sd), "torch's AdamW": plain.state_dict()}.items():
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+            pytest.fail(f"{name} was not refused")
+        assert same(opt.state_dict(), before), name
+        assert [p is q for p, q in zip(opt.param_groups[0]["params"], ps)] == [True, True]
+    eight = AdamW(params(), state_bits=8)
+    with pytest.raises(ValueError, match="saved moments"):
+        eight.load_state_dict(sd)
+    short = saved_state(eight, [1, 1], 8)
+    short["state"][0]["exp_avg_scale"] = torch.zeros(1, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="exp_avg_scale"):
+        eight.load_state_dict(short)
+    assert not eight.state

@@ -8,6 +8,8 @@ reads them.
 
 from __future__ import annotations
 
+import collections
+import copy
 from typing import Any, Dict, List, Optional, Tuple
 
 import torch
@@ -125,32 +127,65 @@ class AdamW(torch.optim.Optimizer):
                 s["master"].copy_(p)
 
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
-        """State tensors keep the dtypes they were saved with (the base class casts them to the
-        parameter's)."""
-        ours = [p for g in self.param_groups for p in g["params"]]
-        bits = [g["state_bits"] for g in self.param_groups for _ in g["params"]]
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        saved = state_dict["state"]
-        for p, b, i in zip(ours, bits, ids):
-            s = saved.get(i)
-            if s is None:
-                continue
-            dtype = torch.float32 if b == 32 else torch.uint8
-            if s["exp_avg"].dtype != dtype or s["exp_avg"].shape != p.shape:
-                raise ValueError(
-                    f"saved moments are {s['exp_avg'].dtype} {tuple(s['exp_avg'].shape)}; this optimizer holds {dtype} "
-                    f"{tuple(p.shape)}"
-                )
-        super().load_state_dict(state_dict)
+        """The state of :meth:`state_dict`; what does not fit this optimizer (another optimizer's state, other
+        shapes, moments in other bits) raises ``ValueError`` and leaves it as it was.  State tensors keep
+        the dtypes they were saved with."""
+        state_dict = state_dict.copy()
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
+        saved, groups = state_dict["state"], copy.deepcopy(state_dict["param_groups"])
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("the saved parameter groups differ from this optimizer's in number or size")
+        loaded: List[Tuple[torch.Tensor, Dict[str, Any]]] = []
+        for mine, group in zip(self.param_groups, groups):
+            missing = [k for k in self._GROUP_KEYS if k not in group]
+            if missing:
+                raise ValueError(f"not a state of this optimizer: its parameter groups have no {', '.join(missing)}")
+            ops._adamw_hyper(group["betas"], group["eps"], group["weight_decay"])
+            for p, i in zip(mine["params"], group["params"]):
+                if saved.get(i):
+                    self._check_state(mine, p, saved[i])
+                    loaded.append((p, saved[i]))
+        # from here on nothing is refused
+        ids = {i for g in groups for i in g["params"]}
+        state: Dict[Any, Any] = collections.defaultdict(dict)
+        state.update((k, v) for k, v in saved.items() if k not in ids)
         self._next_base = 0
-        for p, i in zip(ours, ids):
-            s = saved.get(i)
-            if s is None:
-                continue
-            self.state[p] = {k: v.detach().to(p.device, copy=True).contiguous() if isinstance(v, torch.Tensor) else v
-                             for k, v in s.items()}
+        for p, s in loaded:
+            state[p] = {k: v.detach().to(p.device, copy=True).contiguous() if isinstance(v, torch.Tensor) else v
+                        for k, v in s.items()}
             end = s["index_base"] + -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
             self._next_base = max(self._next_base, end)
+        for mine, group in zip(self.param_groups, groups):
+            group["params"] = mine["params"]
+            if "param_names" in mine:
+                group.setdefault("param_names", mine["param_names"])
+        self.__setstate__({"state": state, "param_groups": groups})
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
+
+    _GROUP_KEYS = ("lr", "betas", "eps", "weight_decay", "state_bits", "master_weights", "seed", "step")
+
+    @staticmethod
+    def _check_state(group: Dict[str, Any], p: torch.Tensor, s: Dict[str, Any]) -> None:
+        missing = [k for k in ("step", "index_base", "exp_avg", "exp_avg_sq") if k not in s]
+        if missing:
+            raise ValueError(f"not a state of this optimizer: a parameter's state has no {', '.join(missing)}")
+        blocks = -(-p.numel() // ops.ADAMW_BLOCK)
+        dtype = torch.float32 if group["state_bits"] == 32 else torch.uint8
+        want = {"exp_avg": (dtype, p.shape), "exp_avg_sq": (dtype, p.shape)}
+        if dtype is torch.uint8:
+            want.update({"exp_avg_scale": (dtype, (blocks,)), "exp_avg_sq_scale": (dtype, (blocks,))})
+        if "master" in s:
+            want["master"] = (torch.float32, p.shape)
+        for name, (kind, shape) in want.items():
+            t = s.get(name)
+            if not isinstance(t, torch.Tensor) or t.dtype != kind or t.shape != torch.Size(shape):
+                found = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
+                raise ValueError(f"saved moments are unlike this optimizer's: {name} is {found}; it holds {kind} {tuple(shape)}")
+        if s["index_base"] < 0 or s["index_base"] % ops.ADAMW_BLOCK:
+            raise ValueError(f"index_base must be a multiple of {ops.ADAMW_BLOCK}; got {s['index_base']}")
 
     # -- the step ------------------------------------------------------------
     @torch.no_grad()
