@@ -127,3 +127,42 @@ def test_a_refused_state_leaves_the_optimizer_as_it_was(AdamW):
     with pytest.raises(ValueError, match="exp_avg_scale"):
         eight.load_state_dict(short)
     assert not eight.state
+
+
+def test_the_count_of_steps_moves_between_host_and_device(AdamW):
+    """Without ``capturable`` each parameter counts, with it the group does, on the device: a state saved
+    one way and loaded the other goes on counting."""
+    host, dev = AdamW(params()), AdamW(params(), capturable=True)
+    dev.load_state_dict(saved_state(host, [5, 5]))
+    step = dev.param_groups[0]["step"]
+    assert step.dtype == torch.int64 and step.shape == () and int(step) == 5
+    assert [dev.state[p]["step"] for p in dev.param_groups[0]["params"]] == [0, 0]  # one call for all of a group
+    back = AdamW(params())
+    back.load_state_dict(dev.state_dict())
+    assert back.param_groups[0]["step"] is None
+    assert [back.state[p]["step"] for p in back.param_groups[0]["params"]] == [5, 5]
+    # the same way round nothing changes, and the copy counts alone
+    again = AdamW(params(), capturable=True)
+    again.load_state_dict(dev.state_dict())
+    step.add_(1)
+    assert int(again.param_groups[0]["step"]) == 5
+    one = AdamW(params())
+    one.load_state_dict(saved_state(one, [5, 2]))
+    assert [one.state[p]["step"] for p in one.param_groups[0]["params"]] == [5, 2]
+
+
+def test_counts_that_one_number_cannot_hold(AdamW):
+    dev = AdamW(params(), capturable=True)
+    with pytest.raises(ValueError, match="number of steps per group"):
+        dev.load_state_dict(saved_state(AdamW(params()), [5, 2]))
+    assert not dev.state and dev.param_groups[0]["step"] is None
+    # a parameter that never had a gradient has no state, and groups count apart
+    dev.load_state_dict(saved_state(AdamW(params()), [5, None]))
+    assert int(dev.param_groups[0]["step"]) == 5
+    def two(**kw):
+        return AdamW([{"params": [p]} for p in params()], **kw)
+    dev = two(capturable=True)
+    dev.load_state_dict(saved_state(two(), [5, 2]))
+    assert [int(g["step"]) for g in dev.param_groups] == [5, 2]
+    dev.load_state_dict(saved_state(two(), [None, None]))
+    assert [g["step"] for g in dev.param_groups] == [None, None]

@@ -137,24 +137,26 @@ class AdamW(torch.optim.Optimizer):
         saved, groups = state_dict["state"], copy.deepcopy(state_dict["param_groups"])
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the saved parameter groups differ from this optimizer's in number or size")
-        loaded: List[Tuple[torch.Tensor, Dict[str, Any]]] = []
+        loaded: List[Tuple[torch.Tensor, Dict[str, Any], int]] = []
         for mine, group in zip(self.param_groups, groups):
             missing = [k for k in self._GROUP_KEYS if k not in group]
             if missing:
                 raise ValueError(f"not a state of this optimizer: its parameter groups have no {', '.join(missing)}")
             ops._adamw_hyper(group["betas"], group["eps"], group["weight_decay"])
-            for p, i in zip(mine["params"], group["params"]):
-                if saved.get(i):
-                    self._check_state(mine, p, saved[i])
-                    loaded.append((p, saved[i]))
+            states = [(p, saved[i]) for p, i in zip(mine["params"], group["params"]) if saved.get(i)]
+            for p, s in states:
+                self._check_state(mine, p, s)
+            counts = self._counts(mine["params"], group, [s for _, s in states])
+            loaded += [(p, s, n) for (p, s), n in zip(states, counts)]
         # from here on nothing is refused
         ids = {i for g in groups for i in g["params"]}
         state: Dict[Any, Any] = collections.defaultdict(dict)
         state.update((k, v) for k, v in saved.items() if k not in ids)
         self._next_base = 0
-        for p, s in loaded:
+        for p, s, count in loaded:
             state[p] = {k: v.detach().to(p.device, copy=True).contiguous() if isinstance(v, torch.Tensor) else v
                         for k, v in s.items()}
+            state[p]["step"] = count
             end = s["index_base"] + -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
             self._next_base = max(self._next_base, end)
         for mine, group in zip(self.param_groups, groups):
@@ -164,6 +166,21 @@ class AdamW(torch.optim.Optimizer):
         self.__setstate__({"state": state, "param_groups": groups})
         for hook in self._optimizer_load_state_dict_post_hooks.values():
             hook(self)
+
+    def _counts(self, params: List[torch.Tensor], group: Dict[str, Any], states: List[Dict[str, Any]]) -> List[int]:
+        """Where this optimizer keeps the count of steps: ``group["step"]`` on the device with ``capturable`` (the
+        states then hold 0), else one number per state.  A count saved in the other place moves over."""
+        count, counts = group["step"], [int(s["step"]) for s in states]
+        if not self.capturable:
+            group["step"] = None
+            return counts if count is None else [int(count)] * len(states)
+        if count is None and counts:
+            if len(set(counts)) > 1:
+                raise ValueError(f"capturable=True counts one number of steps per group; the saved parameters have {sorted(set(counts))}")
+            count = counts[0]
+        if count is not None:
+            group["step"] = torch.tensor(int(count), dtype=torch.int64, device=params[0].device if params else None)
+        return [0] * len(states)
 
     _GROUP_KEYS = ("lr", "betas", "eps", "weight_decay", "state_bits", "master_weights", "seed", "step")
 
