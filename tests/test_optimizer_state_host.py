@@ -166,3 +166,22 @@ def test_counts_that_one_number_cannot_hold(AdamW):
     assert [int(g["step"]) for g in dev.param_groups] == [5, 2]
     dev.load_state_dict(saved_state(two(), [None, None]))
     assert [g["step"] for g in dev.param_groups] == [None, None]
+
+
+def test_how_a_state_is_held_stays_the_optimizers_choice(AdamW):
+    """Bits and masters that differ are refused where a state has them, and never overwritten."""
+    def build(**kw):
+        return AdamW(params(torch.bfloat16), **kw)
+    for mine, theirs in ((True, False), (False, True)):
+        opt = build(master_weights=mine)
+        with pytest.raises(ValueError, match="master"):
+            opt.load_state_dict(saved_state(build(master_weights=theirs), [2, 2], master=theirs))
+        assert opt.param_groups[0]["master_weights"] is mine and not opt.state
+    # before its first step an optimizer has no state that could differ
+    opt = build(master_weights=True, state_bits=8)
+    opt.load_state_dict(build(lr=0.5).state_dict())
+    assert (opt.param_groups[0]["master_weights"], opt.param_groups[0]["state_bits"], opt.param_groups[0]["lr"]) == (True, 8, 0.5)
+    # fp32 parameters have no masters under either setting
+    opt = AdamW(params(), master_weights=True)
+    opt.load_state_dict(saved_state(AdamW(params()), [2, 2]))
+    assert opt.param_groups[0]["master_weights"] is True and len(opt.state) == 2

@@ -128,8 +128,9 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
         """The state of :meth:`state_dict`; what does not fit this optimizer (another optimizer's state, other
-        shapes, moments in other bits) raises ``ValueError`` and leaves it as it was.  State tensors keep
-        the dtypes they were saved with."""
+        shapes, moments in other bits, masters on one side only) raises ``ValueError`` and leaves it as it was.
+        The groups take the saved rates and constants; how a state is held (``state_bits``,
+        ``master_weights``) stays this optimizer's choice."""
         state_dict = state_dict.copy()
         for hook in self._optimizer_load_state_dict_pre_hooks.values():
             changed = hook(self, state_dict)
@@ -143,6 +144,8 @@ class AdamW(torch.optim.Optimizer):
             if missing:
                 raise ValueError(f"not a state of this optimizer: its parameter groups have no {', '.join(missing)}")
             ops._adamw_hyper(group["betas"], group["eps"], group["weight_decay"])
+            for k in ("state_bits", "master_weights"):
+                group[k] = mine[k]
             states = [(p, saved[i]) for p, i in zip(mine["params"], group["params"]) if saved.get(i)]
             for p, s in states:
                 self._check_state(mine, p, s)
@@ -194,13 +197,15 @@ class AdamW(torch.optim.Optimizer):
         want = {"exp_avg": (dtype, p.shape), "exp_avg_sq": (dtype, p.shape)}
         if dtype is torch.uint8:
             want.update({"exp_avg_scale": (dtype, (blocks,)), "exp_avg_sq_scale": (dtype, (blocks,))})
-        if "master" in s:
+        if group["master_weights"] and p.dtype is not torch.float32:
             want["master"] = (torch.float32, p.shape)
         for name, (kind, shape) in want.items():
             t = s.get(name)
             if not isinstance(t, torch.Tensor) or t.dtype != kind or t.shape != torch.Size(shape):
                 found = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
                 raise ValueError(f"saved moments are unlike this optimizer's: {name} is {found}; it holds {kind} {tuple(shape)}")
+        if "master" in s and "master" not in want:
+            raise ValueError("the saved state has fp32 masters; this optimizer (master_weights=False) would lose them")
         if s["index_base"] < 0 or s["index_base"] % ops.ADAMW_BLOCK:
             raise ValueError(f"index_base must be a multiple of {ops.ADAMW_BLOCK}; got {s['index_base']}")
 
