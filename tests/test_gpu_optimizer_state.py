@@ -48,3 +48,28 @@ def test_a_state_moves_between_host_and_device_counts(dev, bits, first):
             for name in ("exp_avg", "exp_avg_sq", "master"):
                 assert torch.equal(a.state[p][name], b.state[q][name]), (k, name)
     assert not math.isnan(float(b.grad_norm))
+
+
+def test_a_checkpoint_mapped_to_the_cpu(dev):
+    """Saved with a tensor rate, read back onto the CPU: the step goes on where the parameters are."""
+    import io
+
+    from unirl_amd.train import AdamW
+
+    def build(ps):
+        return AdamW(ps, lr=torch.tensor(1e-2, device=dev), capturable=True, state_bits=8)
+
+    ours = model(torch.float32, dev)
+    a = build(ours)
+    set_grads(ours, 0)
+    a.step()
+    twin = copied(ours)
+    buf = io.BytesIO()
+    torch.save(a.state_dict(), buf)
+    buf.seek(0)
+    b = build(twin)
+    b.load_state_dict(torch.load(buf, map_location="cpu", weights_only=True))
+    for ps, opt in ((ours, a), (twin, b)):
+        set_grads(ps, 1)
+        opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ours, twin))

@@ -185,3 +185,18 @@ def test_how_a_state_is_held_stays_the_optimizers_choice(AdamW):
     opt = AdamW(params(), master_weights=True)
     opt.load_state_dict(saved_state(AdamW(params()), [2, 2]))
     assert opt.param_groups[0]["master_weights"] is True and len(opt.state) == 2
+
+
+def test_a_tensor_rate_comes_to_the_parameters(AdamW):
+    """A checkpoint mapped to the CPU holds its rate there; the step needs it where the parameters are.
+    (The meta device stands for another one.)"""
+    for capturable in (True, False):
+        opt = AdamW(params(device="meta"), capturable=capturable)
+        sd = copy.deepcopy(opt.state_dict())
+        sd["param_groups"][0]["lr"] = torch.tensor(0.5)
+        opt.load_state_dict(sd)
+        lr = opt.param_groups[0]["lr"]
+        if capturable:
+            assert lr.device.type == "meta" and lr.dtype == torch.float32
+        else:
+            assert lr == 0.5 and isinstance(lr, float)

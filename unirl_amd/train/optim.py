@@ -146,6 +146,9 @@ class AdamW(torch.optim.Optimizer):
             ops._adamw_hyper(group["betas"], group["eps"], group["weight_decay"])
             for k in ("state_bits", "master_weights"):
                 group[k] = mine[k]
+            if isinstance(group["lr"], torch.Tensor):  # where the parameters are; a number where the host counts
+                group["lr"] = (group["lr"].to(mine["params"][0].device if mine["params"] else None, torch.float32)
+                               if self.capturable else float(group["lr"]))
             states = [(p, saved[i]) for p, i in zip(mine["params"], group["params"]) if saved.get(i)]
             for p, s in states:
                 self._check_state(mine, p, s)
