@@ -73,3 +73,47 @@ def test_a_checkpoint_mapped_to_the_cpu(dev):
         set_grads(ps, 1)
         opt.step()
     assert all(torch.equal(p, q) for p, q in zip(ours, twin))
+
+
+def test_a_captured_step_goes_on_with_a_loaded_state(dev):
+    """Captured, trained on, then set back to a state saved before: every replay gives what an optimizer that was
+    loaded with that state and never captured gives."""
+    import copy
+
+    from unirl_amd.train import AdamW
+
+    kw = dict(state_bits=8, master_weights=True, max_grad_norm=1.0, capturable=True, seed=3)
+    lr = torch.tensor(1e-2, device=dev)
+    ours = model(torch.bfloat16, dev)
+    a = AdamW(ours, lr=lr, **kw)
+    set_grads(ours, 0)
+    grads = [p.grad for p in ours]
+    a.step()
+    saved = copy.deepcopy(a.state_dict())
+    twin = copied(ours)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        a.step()
+    lr.fill_(3e-2)
+    for _ in range(2):
+        graph.replay()
+    a.load_state_dict(saved)
+    assert float(lr) == float(torch.tensor(1e-2))
+    with torch.no_grad():
+        for p, q in zip(ours, twin):
+            p.copy_(q)
+    b = AdamW(twin, lr=torch.tensor(1e-2, device=dev), **kw)
+    b.load_state_dict(saved)
+    junk = [torch.full((1 << 16,), 255, dtype=torch.uint8, device=dev) for _ in range(16)]  # takes what was freed
+    for k in range(1, 5):
+        set_grads(twin, k)
+        for g, q in zip(grads, twin):
+            g.copy_(q.grad)
+        graph.replay()
+        b.step()
+        torch.cuda.synchronize()
+        for p, q in zip(ours, twin):
+            assert torch.equal(p, q), k
+    assert all(bool((j == 255).all()) for j in junk)
+    assert int(a.param_groups[0]["step"]) == int(b.param_groups[0]["step"]) == 5

@@ -164,8 +164,9 @@ def test_counts_that_one_number_cannot_hold(AdamW):
     dev = two(capturable=True)
     dev.load_state_dict(saved_state(two(), [5, 2]))
     assert [int(g["step"]) for g in dev.param_groups] == [5, 2]
-    dev.load_state_dict(saved_state(two(), [None, None]))
-    assert [g["step"] for g in dev.param_groups] == [None, None]
+    fresh = two(capturable=True)
+    fresh.load_state_dict(saved_state(two(), [None, None]))
+    assert [g["step"] for g in fresh.param_groups] == [None, None]
 
 
 def test_how_a_state_is_held_stays_the_optimizers_choice(AdamW):
@@ -200,3 +201,55 @@ def test_a_tensor_rate_comes_to_the_parameters(AdamW):
             assert lr.device.type == "meta" and lr.dtype == torch.float32
         else:
             assert lr == 0.5 and isinstance(lr, float)
+
+
+def held(opt):
+    """Every tensor that a captured step of ``opt`` would read or write beside parameters and gradients."""
+    return [t for p in opt.param_groups[0]["params"] for t in opt.state[p].values() if isinstance(t, torch.Tensor)] + [
+        g[k] for g in opt.param_groups for k in ("step", "lr") if isinstance(g[k], torch.Tensor)] + list(opt._controls.values())
+
+
+def test_what_a_captured_step_holds_is_written_in_place(AdamW):
+    lr = torch.tensor(0.25)
+    opt = AdamW(params(torch.bfloat16), lr=lr, state_bits=8, master_weights=True, capturable=True)
+    opt._controls[0] = torch.zeros(32, dtype=torch.uint8)
+    opt.load_state_dict(saved_state(opt, [3, 3], 8, master=True))
+    before = held(opt)
+    assert len(before) == 2 * 5 + 3
+    sd = saved_state(opt, [4, 4], 8, master=True)
+    sd["param_groups"][0].update(lr=torch.tensor(0.125), step=torch.tensor(7))
+    sd["state"][1]["exp_avg"] += 1
+    opt.load_state_dict(sd)
+    assert all(a is b for a, b in zip(held(opt), before)) and lr == 0.125
+    assert int(opt.param_groups[0]["step"]) == 7
+    assert torch.equal(opt.state[opt.param_groups[0]["params"][1]]["exp_avg"], sd["state"][1]["exp_avg"])
+    # its own tensors, the two parameters' masters exchanged: read before they are written
+    ps = opt.param_groups[0]["params"]
+    a = AdamW([ps[0], torch.nn.Parameter(ps[0].detach().clone())], capturable=True, master_weights=True)
+    a.load_state_dict(saved_state(a, [1, 1], master=True))
+    mine = a.state_dict()
+    mine["state"][1]["master"].fill_(9.0)
+    mine["state"] = {0: dict(mine["state"][1]), 1: dict(mine["state"][0])}
+    a.load_state_dict(mine)
+    assert [float(a.state[p]["master"].mean()) for p in a.param_groups[0]["params"]] == [9.0, 0.5]
+    # a state from before the first step: zeros, and masters as the parameters are
+    with torch.no_grad():
+        ps[0].fill_(2.0)
+    before = held(opt)
+    opt.load_state_dict(AdamW(params(torch.bfloat16), lr=0.5, state_bits=8, master_weights=True, capturable=True).state_dict())
+    assert all(a is b for a, b in zip(held(opt), before)) and lr == 0.5
+    s = opt.state[ps[0]]
+    assert int(opt.param_groups[0]["step"]) == 0 and bool((s["master"] == 2.0).all())
+    assert not any(s[k].any() for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"))
+    bases = [opt.state[p]["index_base"] for p in ps]
+    assert len(set(bases)) == 2 and opt._next_base == 512 + 256
+
+
+def test_groups_that_share_a_tensor_rate_load_rates_of_their_own(AdamW):
+    lr = torch.tensor(0.25)
+    opt = AdamW([{"params": [p]} for p in params()], lr=lr, capturable=True)
+    sd = copy.deepcopy(opt.state_dict())
+    sd["param_groups"][0]["lr"], sd["param_groups"][1]["lr"] = 0.5, torch.tensor(0.125)
+    opt.load_state_dict(sd)
+    assert [float(g["lr"]) for g in opt.param_groups] == [0.5, 0.125] and lr == 0.25
+    assert all(isinstance(g["lr"], torch.Tensor) for g in opt.param_groups)

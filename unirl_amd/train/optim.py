@@ -18,6 +18,13 @@ from .. import _native as N
 from .. import ops
 
 
+def _placed(saved: torch.Tensor, held: Any, device: torch.device) -> torch.Tensor:
+    """A copy of ``saved`` on ``device``, in the tensor ``held`` where that is of its kind."""
+    if isinstance(held, torch.Tensor) and (held.shape, held.dtype, held.device) == (saved.shape, saved.dtype, device):
+        return held.copy_(saved)
+    return saved.detach().to(device, copy=True).contiguous()
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW``'s update (decoupled weight decay) with fused kernels.
 
@@ -102,7 +109,7 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: run one step before capturing: the state would be made anew by every replay")
         blocks = -(-p.numel() // ops.ADAMW_BLOCK)
         state: Dict[str, Any] = {"step": 0, "index_base": self._next_base}
-        self._next_base += blocks * ops.ADAMW_BLOCK
+        self._next_base += self._indices(p)
         dtype = torch.float32 if group["state_bits"] == 32 else torch.uint8
         for name in ("exp_avg", "exp_avg_sq"):
             state[name] = torch.zeros(p.shape, dtype=dtype, device=p.device)
@@ -126,11 +133,13 @@ class AdamW(torch.optim.Optimizer):
             if "master" in s:
                 s["master"].copy_(p)
 
+    @torch.no_grad()
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
         """The state of :meth:`state_dict`; what does not fit this optimizer (another optimizer's state, other
         shapes, moments in other bits, masters on one side only) raises ``ValueError`` and leaves it as it was.
         The groups take the saved rates and constants; how a state is held (``state_bits``,
-        ``master_weights``) stays this optimizer's choice."""
+        ``master_weights``) stays this optimizer's choice.  States, counts and tensor rates that are
+        already there are written in place, so that a captured step goes on with what was loaded."""
         state_dict = state_dict.copy()
         for hook in self._optimizer_load_state_dict_pre_hooks.values():
             changed = hook(self, state_dict)
@@ -138,6 +147,7 @@ class AdamW(torch.optim.Optimizer):
         saved, groups = state_dict["state"], copy.deepcopy(state_dict["param_groups"])
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the saved parameter groups differ from this optimizer's in number or size")
+        rates = [float(g["lr"]) for g in groups if "lr" in g]
         loaded: List[Tuple[torch.Tensor, Dict[str, Any], int]] = []
         for mine, group in zip(self.param_groups, groups):
             missing = [k for k in self._GROUP_KEYS if k not in group]
@@ -152,28 +162,46 @@ class AdamW(torch.optim.Optimizer):
             states = [(p, saved[i]) for p, i in zip(mine["params"], group["params"]) if saved.get(i)]
             for p, s in states:
                 self._check_state(mine, p, s)
-            counts = self._counts(mine["params"], group, [s for _, s in states])
+            counts = self._counts(mine, group, [s for _, s in states])
             loaded += [(p, s, n) for (p, s), n in zip(states, counts)]
         # from here on nothing is refused
         ids = {i for g in groups for i in g["params"]}
         state: Dict[Any, Any] = collections.defaultdict(dict)
         state.update((k, v) for k, v in saved.items() if k not in ids)
+        # saved tensors that are this optimizer's own may be written before they are read
+        own = {t.data_ptr() for s in self.state.values() for t in s.values() if isinstance(t, torch.Tensor)}
+        loaded = [(p, {k: v.clone() if isinstance(v, torch.Tensor) and v.data_ptr() in own else v for k, v in s.items()}, n)
+                  for p, s, n in loaded]
         self._next_base = 0
         for p, s, count in loaded:
-            state[p] = {k: v.detach().to(p.device, copy=True).contiguous() if isinstance(v, torch.Tensor) else v
-                        for k, v in s.items()}
+            old = self.state.get(p, {})
+            state[p] = {k: _placed(v, old.get(k), p.device) if isinstance(v, torch.Tensor) else v for k, v in s.items()}
             state[p]["step"] = count
-            end = s["index_base"] + -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
-            self._next_base = max(self._next_base, end)
-        for mine, group in zip(self.param_groups, groups):
+            self._next_base = max(self._next_base, s["index_base"] + self._indices(p))
+        for mine, group, rate in zip(self.param_groups, groups, rates):
+            for p in mine["params"]:
+                if self.capturable and self.state.get(p) and p not in state:  # a captured step may hold it
+                    state[p] = self.state[p]
+                    for k, v in state[p].items():
+                        if isinstance(v, torch.Tensor):
+                            v.copy_(p) if k == "master" else v.zero_()
+                    state[p]["index_base"] = self._next_base
+                    self._next_base += self._indices(p)
             group["params"] = mine["params"]
             if "param_names" in mine:
                 group.setdefault("param_names", mine["param_names"])
+            if isinstance(group["step"], torch.Tensor):
+                group["step"] = _placed(group["step"], mine["step"], group["step"].device)
+            if self.capturable and isinstance(mine["lr"], torch.Tensor):  # may be the rate of several groups
+                one = len({r for g, r in zip(self.param_groups, rates) if g["lr"] is mine["lr"]}) == 1
+                group["lr"] = mine["lr"].fill_(rate) if one else torch.full_like(mine["lr"], rate)
+        controls = self._controls
         self.__setstate__({"state": state, "param_groups": groups})
+        self._controls = controls
         for hook in self._optimizer_load_state_dict_post_hooks.values():
             hook(self)
 
-    def _counts(self, params: List[torch.Tensor], group: Dict[str, Any], states: List[Dict[str, Any]]) -> List[int]:
+    def _counts(self, mine: Dict[str, Any], group: Dict[str, Any], states: List[Dict[str, Any]]) -> List[int]:
         """Where this optimizer keeps the count of steps: ``group["step"]`` on the device with ``capturable`` (the
         states then hold 0), else one number per state.  A count saved in the other place moves over."""
         count, counts = group["step"], [int(s["step"]) for s in states]
@@ -184,9 +212,15 @@ class AdamW(torch.optim.Optimizer):
             if len(set(counts)) > 1:
                 raise ValueError(f"capturable=True counts one number of steps per group; the saved parameters have {sorted(set(counts))}")
             count = counts[0]
-        if count is not None:
-            group["step"] = torch.tensor(int(count), dtype=torch.int64, device=params[0].device if params else None)
+        if count is not None or mine["step"] is not None:
+            device = mine["params"][0].device if mine["params"] else None
+            group["step"] = torch.tensor(int(count or 0), dtype=torch.int64, device=device)
         return [0] * len(states)
+
+    @staticmethod
+    def _indices(p: torch.Tensor) -> int:
+        """Dither positions of a parameter's elements: whole blocks."""
+        return -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
 
     _GROUP_KEYS = ("lr", "betas", "eps", "weight_decay", "state_bits", "master_weights", "seed", "step")
 
