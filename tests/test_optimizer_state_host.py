@@ -253,3 +253,12 @@ def test_groups_that_share_a_tensor_rate_load_rates_of_their_own(AdamW):
     opt.load_state_dict(sd)
     assert [float(g["lr"]) for g in opt.param_groups] == [0.5, 0.125] and lr == 0.25
     assert all(isinstance(g["lr"], torch.Tensor) for g in opt.param_groups)
+
+
+def test_moments_of_a_parameter_without_a_state(AdamW):
+    """Asking leaves nothing behind: an empty entry would be saved with the others."""
+    ps = params()
+    opt = AdamW(ps)
+    with pytest.raises(ValueError, match="no state"):
+        opt.moments(ps[0])
+    assert not opt.state and opt.state_dict()["state"] == {}

@@ -121,7 +121,9 @@ class AdamW(torch.optim.Optimizer):
 
     def moments(self, p: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """``(exp_avg, exp_avg_sq)`` of a parameter as fp32 values, whatever they are held in."""
-        s = self.state[p]
+        s = self.state.get(p)  # a look must not leave an entry behind
+        if not s:
+            raise ValueError("the parameter has no state: it had no gradient in any step so far")
         if "exp_avg_scale" not in s:
             return s["exp_avg"], s["exp_avg_sq"]
         return ops.adamw_moments(s["exp_avg"], s["exp_avg_sq"], s["exp_avg_scale"], s["exp_avg_sq_scale"])
