@@ -262,3 +262,19 @@ def test_moments_of_a_parameter_without_a_state(AdamW):
     with pytest.raises(ValueError, match="no state"):
         opt.moments(ps[0])
     assert not opt.state and opt.state_dict()["state"] == {}
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate parameters")
+def test_a_refused_group_is_not_added(AdamW):
+    opt = AdamW(params())
+    p = torch.nn.Parameter(torch.zeros(4, 6))
+    for bad in (dict(params=[p], state_bits=4), dict(params=[p], betas=(1.0, 0.9)), dict(params=[p, p]),
+                dict(params=[torch.nn.Parameter(torch.zeros(6, 4).t())])):
+        with pytest.raises(ValueError):
+            opt.add_param_group(bad)
+        assert len(opt.param_groups) == 1
+    with pytest.raises(TypeError):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2, dtype=torch.float64))]))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[p]))
+    assert len(opt.param_groups) == 2

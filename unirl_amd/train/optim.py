@@ -83,13 +83,19 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, param_group: Dict[str, Any]) -> None:
         super().add_param_group(param_group)
         group = self.param_groups[-1]
-        ops._adamw_hyper(group["betas"], group["eps"], group["weight_decay"])
-        if group["state_bits"] not in (8, 32):
-            raise ValueError(f"state_bits must be 8 or 32; got {group['state_bits']}")
-        for p in group["params"]:
-            N.dtype_code(p.dtype)
-            if not p.is_contiguous():
-                raise ValueError(f"parameters must be contiguous; got strides {p.stride()} of {tuple(p.shape)}")
+        try:
+            ops._adamw_hyper(group["betas"], group["eps"], group["weight_decay"])
+            if group["state_bits"] not in (8, 32):
+                raise ValueError(f"state_bits must be 8 or 32; got {group['state_bits']}")
+            if len(set(group["params"])) != len(group["params"]):
+                raise ValueError("a parameter appears more than once in its group")
+            for p in group["params"]:
+                N.dtype_code(p.dtype)
+                if not p.is_contiguous():
+                    raise ValueError(f"parameters must be contiguous; got strides {p.stride()} of {tuple(p.shape)}")
+        except Exception:
+            self.param_groups.pop()
+            raise
 
     # -- copies and pickles: the base class keeps defaults, state and groups alone ---------------------
     _OPTIONS = ("max_grad_norm", "skip_nonfinite", "capturable", "_next_base")
