@@ -117,3 +117,26 @@ def test_a_captured_step_goes_on_with_a_loaded_state(dev):
             assert torch.equal(p, q), k
     assert all(bool((j == 255).all()) for j in junk)
     assert int(a.param_groups[0]["step"]) == int(b.param_groups[0]["step"]) == 5
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_leaves_every_group_as_it_was(dev, capturable):
+    """The second group lies on the CPU, where there is no kernel: the first is not stepped either."""
+    from unirl_amd.train import AdamW
+
+    ours = model(torch.float32, dev)
+    other = torch.nn.Parameter(torch.zeros(4))
+    opt = AdamW([dict(params=ours), dict(params=[other])], capturable=capturable)
+    set_grads(ours, 0)
+    before = [p.detach().clone() for p in ours]
+    other.grad = torch.ones_like(other)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ours, before))
+    other.grad = None
+    twin = AdamW([dict(params=copied(ours))], capturable=capturable)
+    set_grads(twin.param_groups[0]["params"], 0)
+    opt.step()
+    twin.step()
+    assert all(torch.equal(p, q) for p, q in zip(ours, twin.param_groups[0]["params"]))

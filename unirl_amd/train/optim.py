@@ -43,7 +43,8 @@ class AdamW(torch.optim.Optimizer):
     ``skip_nonfinite`` needs it.  The first step, which makes the state, has to run before the capture.
     Otherwise each parameter counts the steps in which it had a gradient.
 
-    Parameters are contiguous fp32, bf16 or fp16 tensors on a HIP device; sparse gradients are refused.
+    Parameters are contiguous fp32, bf16 or fp16 tensors on a HIP device, one per group (with clipping or
+    ``skip_nonfinite``, one for all groups); sparse gradients are refused.
     """
 
     def __init__(
@@ -110,6 +111,8 @@ class AdamW(torch.optim.Optimizer):
 
     # -- state -------------------------------------------------------------
     def _new_state(self, group: Dict[str, Any], p: torch.Tensor) -> Dict[str, Any]:
+        if p.device != group["params"][0].device:
+            raise ValueError(f"parameters of one group share one device; got {p.device} and {group['params'][0].device}")
         N.require_device(p, "parameter")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: run one step before capturing: the state would be made anew by every replay")
@@ -268,6 +271,18 @@ class AdamW(torch.optim.Optimizer):
         pairs = [[(p, p.grad) for p in group["params"] if p.grad is not None] for group in self.param_groups]
         if any(g.layout is not strided for group in pairs for _, g in group):
             raise RuntimeError("AdamW does not support sparse gradients")
+        counted = not self.capturable
+        # what shares a call: types, master, count of steps; all groups' before the first launch, so that a
+        # state that cannot be made leaves every group as it was
+        work: List[Dict[Any, List[Any]]] = []
+        for group, with_grad in zip(self.param_groups, pairs):
+            buckets: Dict[Any, List[Any]] = {}
+            for p, g in with_grad:
+                s = state_of.get(p)
+                if not s:
+                    s = state_of[p] = self._new_state(group, p)
+                buckets.setdefault((p.dtype, g.dtype, "master" in s, s["step"]), []).append((p, g, s))
+            work.append(buckets)
         self.grad_norm = None
         clip: Dict[str, Any] = {}
         if self.max_grad_norm is not None or self.skip_nonfinite:
@@ -275,16 +290,9 @@ class AdamW(torch.optim.Optimizer):
             if grads:
                 self.grad_norm = ops.grad_norm(grads)
                 clip = dict(grad_norm=self.grad_norm, max_norm=self.max_grad_norm, skip_nonfinite=self.skip_nonfinite)
-        for index, (group, with_grad) in enumerate(zip(self.param_groups, pairs)):
+        for index, (group, with_grad, buckets) in enumerate(zip(self.param_groups, pairs, work)):
             if not with_grad:
                 continue
-            buckets: Dict[Any, List[Any]] = {}  # what shares a call: types, master, count of steps
-            counted = not self.capturable
-            for p, g in with_grad:
-                s = state_of[p]
-                if not s:
-                    s.update(self._new_state(group, p))
-                buckets.setdefault((p.dtype, g.dtype, "master" in s, s["step"]), []).append((p, g, s))
             how: Dict[str, Any] = {}
             if self.capturable:
                 how["control"] = self._advance(index, group, with_grad[0][0].device, clip)
