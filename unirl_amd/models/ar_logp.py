@@ -27,6 +27,18 @@ from .. import ops
 from .norm import layer_norm, rms_norm
 
 
+def _is_altered(module: torch.nn.Module) -> bool:
+    """Whether calling the module does something beside, before or instead of its class's ``forward``: hooks
+    of any kind, or a ``forward`` set on the instance (as offloading and instrumentation wrappers do)."""
+    from torch.nn.modules import module as _m
+
+    return bool(
+        "forward" in vars(module)
+        or module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+        or _m._global_forward_hooks or _m._global_forward_pre_hooks or _m._global_backward_hooks or _m._global_backward_pre_hooks
+    )
+
+
 def _is_plain_linear(lm_head) -> bool:
     """True for an ``nn.Linear`` proper whose output nobody else can be holding: not a subclass
     (a quantised or custom Linear's autograd may save its output) and no forward hook (a hook
@@ -254,16 +266,11 @@ def token_entropy(logits: torch.Tensor, temperature: float = 1.0) -> torch.Tenso
 
 def _apply_final_norm(norm: Callable[[torch.Tensor], torch.Tensor], hidden: torch.Tensor) -> torch.Tensor:
     """``norm(hidden)``; a plain ``nn.RMSNorm`` / ``nn.LayerNorm`` over the last dimension runs as one
-    fused kernel each way.  Subclasses, modules with hooks, other callables and autocast go through
-    their own call."""
-    from torch.nn.modules import module as _m
-
+    fused kernel each way.  Subclasses, modules with hooks or a ``forward`` of their own, other callables and
+    autocast go through their own call."""
     kind = type(norm)
     own = (
-        kind in (torch.nn.RMSNorm, torch.nn.LayerNorm)
-        and not (norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks)
-        and not (_m._global_forward_hooks or _m._global_forward_pre_hooks or _m._global_backward_hooks
-                 or _m._global_backward_pre_hooks)
+        kind in (torch.nn.RMSNorm, torch.nn.LayerNorm) and not _is_altered(norm)
         and tuple(norm.normalized_shape) == (hidden.shape[-1],) and hidden.shape[-1] <= ops.NORM_MAX_DIM
         and hidden.is_cuda and hidden.dtype in _KERNEL_DTYPES and not torch.is_autocast_enabled("cuda")
         and all(p.dtype == hidden.dtype and p.device == hidden.device for p in norm.parameters())
