@@ -39,3 +39,11 @@ def test_an_altered_module_is_called(ar_logp, how):
     finally:
         handle.remove()
     assert not ar_logp._is_altered(torch.nn.RMSNorm(8))
+
+
+@pytest.mark.parametrize("how", alterations())
+def test_an_altered_linear_is_not_plain(ar_logp, how):
+    head = torch.nn.Linear(8, 8)
+    assert ar_logp._is_plain_linear(head)
+    alterations()[how](head)
+    assert not ar_logp._is_plain_linear(head)

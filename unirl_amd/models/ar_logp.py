@@ -42,15 +42,11 @@ def _is_altered(module: torch.nn.Module) -> bool:
 def _is_plain_linear(lm_head) -> bool:
     """True for an ``nn.Linear`` proper whose output nobody else can be holding: not a subclass
     (a quantised or custom Linear's autograd may save its output) and no forward hook (a hook
-    sees, and may keep, the output).  Only then may a gradient be written over the logits."""
-    from torch.nn.modules import module as _m
-
-    return (
-        type(lm_head) is torch.nn.Linear
-        and not lm_head._forward_hooks
-        and not lm_head._forward_hooks_with_kwargs
-        and not _m._global_forward_hooks
-    )
+    sees, and may keep, the output).  Only then may a gradient be written over the logits; and only
+    without hooks in front or in the backward, or a ``forward`` of its own, may the product be computed
+    from the weight without calling the module (the older weight and spectral norms make the weight in a
+    hook in front)."""
+    return type(lm_head) is torch.nn.Linear and not _is_altered(lm_head)
 
 
 class _TokenLogpFn(torch.autograd.Function):
