@@ -341,6 +341,8 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const std::optional<Tensor> weight = optional_of(a[1], "weight"), bias = optional_of(a[2], "bias");
   const double eps = number(a[3]);
   const bool rms = truth(a[4]), unit_offset = truth(a[5]);
+  const auto is_dual = [](const std::optional<Tensor>& t) { return t && t->_fw_grad(0).defined(); };
+  TORCH_CHECK(!is_dual(x) && !is_dual(weight) && !is_dual(bias), "the norm has no forward-mode derivative");
   const auto wants = [](const std::optional<Tensor>& t) { return t && t->requires_grad(); };
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants(weight) || wants(bias)))
     return wrap(NormFunction::apply(x, weight, bias, eps, rms, unit_offset));

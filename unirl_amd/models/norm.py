@@ -8,9 +8,9 @@
 
 The forward keeps the row's mean and reciprocal deviation (8 bytes a row) for the backward, which
 reads ``x`` and ``dy`` once and sums the gain's and bias's gradients in the same pass.  Forward and
-backward are one C++ autograd node (``csrc/torch_host.cpp``); the backward is not differentiable.  A
-backward can be captured into a graph, but not for a leaf over which a graph built on the default stream
-is still alive: that is refused.
+backward are one C++ autograd node (``csrc/torch_host.cpp``); the backward is not differentiable and
+there is no forward-mode derivative (both raise).  A backward can be captured into a graph, but not for a
+leaf over which a graph built on the default stream is still alive: that is refused.
 """
 
 from __future__ import annotations
