@@ -647,7 +647,7 @@ size_t unirl_layer_norm_bwd_scratch_bytes(int64_t groups, int64_t rows, int64_t 
  *             or over all rows ([D]); f32 sums in an order that depends on the shape alone
  * dy: x's dtype, its own strides.  dx (dense), dgain, dbias may each be NULL; without rows dgain and
  * dbias are zero.  scratch: device memory for dgain and dbias, not initialised, of at least
- * unirl_layer_norm_bwd_scratch_bytes(); per_group: at most 65535 groups. */
+ * unirl_layer_norm_bwd_scratch_bytes(); dgain or dbias per_group: at most 65535 groups. */
 int unirl_layer_norm_bwd(const struct unirl_norm_desc* desc, const void* dy, int64_t dy_group_stride,
                          int64_t dy_row_stride, void* dx, void* dgain, void* dbias, int per_group,
                          void* scratch, size_t scratch_bytes, void* stream);

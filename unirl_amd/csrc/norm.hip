@@ -858,7 +858,7 @@ extern "C" int unirl_layer_norm_bwd(const struct unirl_norm_desc* d, const void*
   if (params && !dtype_ok(d->gain_dtype)) return UNIRL_E_DTYPE;
   if (params && (!aligned_to(dgain, dtype_size(d->gain_dtype)) || !aligned_to(dbias, dtype_size(d->gain_dtype))))
     return UNIRL_E_ALIGN;
-  if (per_group && d->groups > kNormMaxGroups) return UNIRL_E_LIMIT;
+  if (params && per_group && d->groups > kNormMaxGroups) return UNIRL_E_LIMIT;  // norm_param_kernel's sets lie in gridDim.y
   hipStream_t s = (hipStream_t)stream;
   const bool empty = d->groups == 0 || d->rows == 0;
   const size_t es = dtype_size(d->dtype);

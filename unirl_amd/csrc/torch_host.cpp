@@ -296,9 +296,14 @@ void refuse_accumulators_outside_a_capture(int8_t device) {
   }
 }
 using torch::autograd::variable_list;
+constexpr int64_t kGradientGroups = 65535;  // of unirl_layer_norm_bwd with dgain or dbias per group
 struct NormFunction : torch::autograd::Function<NormFunction> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight,
                         const std::optional<Tensor>& bias, double eps, bool rms, bool unit_offset) {
+    for (const auto* p : {&weight, &bias})  // what the backward would refuse is refused here
+      TORCH_CHECK_VALUE(!*p || (*p)->dim() < 2 || !(*p)->requires_grad() || (*p)->size(0) <= kGradientGroups,
+                        "gains and biases per group have gradients up to the limit of ", kGradientGroups, " groups; got ",
+                        (*p)->size(0));
     at::AutoDispatchBelowADInplaceOrView no_grad;
     const NormOut o = norm_forward(x, weight, bias, eps, rms, unit_offset, true);
     check(o.rc, "unirl_layer_norm_fwd");

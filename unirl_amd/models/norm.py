@@ -47,7 +47,8 @@ def rms_norm(
 def modulated_layer_norm(x: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """``layer_norm(x[b]) * (1 + scale[b]) + shift[b]`` for ``x [B, ..., D]`` and ``scale``, ``shift`` ``[B, D]``
     (or ``[B, 1, ..., D]``; halves of one projection's output are read in place), in ``x``'s dtype;
-    differentiable in all three, the modulation's gradients summed over each sample's rows."""
+    differentiable in all three, the modulation's gradients summed over each sample's rows (for at most 65535
+    samples)."""
     if x.dim() < 2:
         raise ValueError(f"x must be [B, ..., D]; got {tuple(x.shape)}")
     rows = (x.shape[0], x.shape[-1])
