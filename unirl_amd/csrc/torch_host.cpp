@@ -514,6 +514,6 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_unirl_torch_host", nullptr, -1, m
 
 PyMODINIT_FUNC PyInit__unirl_torch_host(void) {
   PyObject* m = PyModule_Create(&module);
-  if (m) PyModule_AddIntConstant(m, "abi_version", unirl_abi_version());
+  if (m) PyModule_AddIntConstant(m, "abi_version", UNIRL_ABI_VERSION);  // the header's, not the loaded library's
   return m;
 }
