@@ -140,3 +140,18 @@ def test_a_refused_step_leaves_every_group_as_it_was(dev, capturable):
     opt.step()
     twin.step()
     assert all(torch.equal(p, q) for p, q in zip(ours, twin.param_groups[0]["params"]))
+
+
+def test_parameters_made_in_inference_mode(dev):
+    """Weights loaded under inference mode have no version to raise: the step counts once, like any other."""
+    from unirl_amd import ops
+
+    def step(p):
+        m, v = torch.zeros(300, device=dev), torch.zeros(300, device=dev)
+        ops.adamw_step([p], [torch.ones(300, device=dev)], [m], [v], lr=1e-2, step=1)
+        return p
+
+    with torch.inference_mode():
+        p = torch.ones(300, device=dev)
+    assert p.is_inference()
+    assert torch.equal(step(p), step(torch.ones(300, device=dev)))

@@ -495,7 +495,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   TORCH_CHECK_VALUE(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "the same parameter appears more than once");
   const int rc = unirl_adamw_step(table.data(), n, &q, stream_of(params[0]));
   // written behind autograd's back: whoever saved a parameter for a backward has to notice
-  for (int64_t i = 0; i < n; ++i) torch::autograd::impl::bump_version(params[i]);
+  for (int64_t i = 0; i < n; ++i)
+    if (!params[i].is_inference()) torch::autograd::impl::bump_version(params[i]);  // inference tensors have no version
   return PyLong_FromLong(rc);
   END_HANDLE_TH_ERRORS
 }
