@@ -283,7 +283,8 @@ def test_a_refused_group_is_not_added(AdamW):
 def test_a_group_on_two_devices_is_refused(AdamW):
     ps = [torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4, device="meta"))]
     opt = AdamW(ps)
-    ps[1].grad = torch.zeros_like(ps[1])
+    for p in ps:
+        p.grad = torch.zeros_like(p)
     with pytest.raises(ValueError, match="one device"):
         opt.step()
     assert not opt.state

@@ -111,8 +111,6 @@ class AdamW(torch.optim.Optimizer):
 
     # -- state -------------------------------------------------------------
     def _new_state(self, group: Dict[str, Any], p: torch.Tensor) -> Dict[str, Any]:
-        if p.device != group["params"][0].device:
-            raise ValueError(f"parameters of one group share one device; got {p.device} and {group['params'][0].device}")
         N.require_device(p, "parameter")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: run one step before capturing: the state would be made anew by every replay")
@@ -277,9 +275,13 @@ class AdamW(torch.optim.Optimizer):
         work: List[Dict[Any, List[Any]]] = []
         for group, with_grad in zip(self.param_groups, pairs):
             buckets: Dict[Any, List[Any]] = {}
+            known = True
             for p, g in with_grad:
                 s = state_of.get(p)
                 if not s:
+                    if known and len({q.device for q, _ in with_grad}) > 1:
+                        raise ValueError("the parameters of a group that have gradients must share one device")
+                    known = False
                     s = state_of[p] = self._new_state(group, p)
                 buckets.setdefault((p.dtype, g.dtype, "master" in s, s["step"]), []).append((p, g, s))
             work.append(buckets)
