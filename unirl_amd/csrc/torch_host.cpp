@@ -1,7 +1,7 @@
 // Host side of the operators whose call cost is their latency: reading torch tensors (addresses,
 // strides, types) and filling the C ABI's structures in C++ instead of in Python.  288 tensors of an
-// optimizer step cost 440 us of attribute reads in Python and 25 us here; a norm's forward 12 us and
-// 6 us.
+// optimizer step cost 440 us of attribute reads in Python and 29 us here (the whole call of
+// ops.adamw_step); a norm's forward 12 us and 5 us.
 //
 // A CPython module over torch's C++ API; it holds no state and no numerics, checks its tensors, and
 // calls libunirl_hip.so.  Functions return the C ABI's status beside their tensors; the Python layer turns

@@ -338,9 +338,11 @@ def chunked_replay_logp(
     ``TRANSPOSED_HEAD_MIN_ROWS`` rows.
 
     ``final_norm`` is for hidden states taken before the model's last norm: it is applied to the
-    response's rows first.  An ``nn.RMSNorm`` or ``nn.LayerNorm`` over the hidden size runs as one fused
-    kernel forward and one backward (``models.rms_norm`` / ``layer_norm``: fp32 inside, one rounding),
-    any other callable as it is.
+    response's rows first.  An ``nn.RMSNorm`` or ``nn.LayerNorm`` over the hidden size (the class itself, without
+    hooks or a ``forward`` of its own) runs as one fused kernel forward and one backward
+    (``models.rms_norm`` / ``layer_norm``: fp32 inside, one rounding), any other callable as it is.  The norm
+    of a Qwen3 model is a class of its own and so runs elementwise; ``lambda h: models.rms_norm(h, norm.weight,
+    norm.variance_epsilon)`` runs the kernel, which does not round the normalised row before the gain.
     """
     bsz, t_max = int(resp_hidden.size(0)), int(response_tokens.size(1))
     if t_max == 0:
