@@ -288,3 +288,14 @@ def test_a_group_on_two_devices_is_refused(AdamW):
     with pytest.raises(ValueError, match="one device"):
         opt.step()
     assert not opt.state
+
+
+def test_a_group_saved_without_its_empty_count(AdamW):
+    """Tools that drop entries that are None leave out the group's count where the states have theirs."""
+    for capturable in (False, True):
+        opt = AdamW(params(), capturable=capturable)
+        sd = saved_state(opt, [5, 5])
+        del sd["param_groups"][0]["step"]
+        opt.load_state_dict(sd)
+        got = opt.param_groups[0]["step"]
+        assert int(got) == 5 if capturable else got is None

@@ -213,7 +213,7 @@ class AdamW(torch.optim.Optimizer):
     def _counts(self, mine: Dict[str, Any], group: Dict[str, Any], states: List[Dict[str, Any]]) -> List[int]:
         """Where this optimizer keeps the count of steps: ``group["step"]`` on the device with ``capturable`` (the
         states then hold 0), else one number per state.  A count saved in the other place moves over."""
-        count, counts = group["step"], [int(s["step"]) for s in states]
+        count, counts = group.setdefault("step", None), [int(s["step"]) for s in states]
         if not self.capturable:
             group["step"] = None
             return counts if count is None else [int(count)] * len(states)
@@ -231,7 +231,7 @@ class AdamW(torch.optim.Optimizer):
         """Dither positions of a parameter's elements: whole blocks."""
         return -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
 
-    _GROUP_KEYS = ("lr", "betas", "eps", "weight_decay", "state_bits", "master_weights", "seed", "step")
+    _GROUP_KEYS = ("lr", "betas", "eps", "weight_decay", "state_bits", "master_weights", "seed")
 
     @staticmethod
     def _check_state(group: Dict[str, Any], p: torch.Tensor, s: Dict[str, Any]) -> None:
